@@ -567,6 +567,149 @@ size_t kdn_scan_workspace_bytes(const KdnScanArgs* args);
 int kdn_scan_fwd(const KdnScanArgs* args, kdn_stream_t stream);
 int kdn_scan_bwd(const KdnScanArgs* args, kdn_stream_t stream);
 
+/* ------------------------------------------------------------------------ *
+ * One new token per sequence through a whole mixer between its projections,
+ * on a pool of per-sequence states updated in place (no counterpart in the
+ * reference, whose mixers reject caches: iso_kdn.py:228-240).  The
+ * single-token form of kdn_short_conv_fwd, the q / k normalisation,
+ * kdn_{iso,diag}_gate_fwd, kdn_{iso,diag}_gain_fwd, kdn_scan_fwd and
+ * kdn_rmsnorm_gated_fwd in one launch, all in fp32.
+ *
+ * Rows are the B sequences of the call; row b uses the states at slots[b]
+ * (slots NULL: slot b).  A slot outside [0, num_slots) marks an idle row: its
+ * output is zero and no state is touched.  A slot may appear once per call.
+ * D = head channels (K = V), 64 or 128.  Activations (qkv, decay_raw,
+ * omega_raw, r_raw, gate, window, y) are bf16 (act_bf16 = 1) or fp32; their
+ * rows are contiguous, with the row strides given (elements); parameters and
+ * states are fp32.  memory and conv_weight must be 16-byte aligned.
+ * Zero-initialise the struct.
+ * ------------------------------------------------------------------------ */
+typedef struct KdnStepArgs {
+  int32_t variant;  /* KDN_ISO or KDN_DIAG */
+  int32_t act_bf16;
+  int32_t swish;    /* output gate: 0 sigmoid(g), 1 g sigmoid(g) */
+  int32_t slots_i64; /* slots are int64 (else int32) */
+  int64_t B, H, D, num_slots;
+  /* the token's projections */
+  const void* qkv;       /* [B, 3*H*D]: q | k | v before the convolution */
+  const void* decay_raw; /* [B, H*D] */
+  const void* omega_raw; /* iso [B, H], diag [B, H*D] */
+  const void* r_raw;     /* [B, H] */
+  const void* gate;      /* [B, H*D] output gate */
+  int64_t qkv_stride, decay_stride, omega_stride, r_stride, gate_stride;
+  /* parameters, fp32 */
+  const float* conv_weight; /* [3*H*D, 4] */
+  const float* A_log;       /* [H] */
+  const float* dt_bias;     /* [H*D] */
+  const float* omega_bias;  /* iso [H] */
+  const float* r_bias;      /* iso [H] */
+  const float* norm_weight; /* nullable [D] */
+  float omega_min, r_min, posterior_scale, eps, scale;
+  /* states */
+  const void* slots;  /* nullable [B] */
+  float* memory;      /* [num_slots, H, D, D], key-major */
+  float* covariance;  /* iso [num_slots, H], diag [num_slots, H, D] */
+  void* window;       /* [num_slots, 3, 3*H*D]: the last three qkv rows, oldest first */
+  void* y;            /* [B, H*D] */
+} KdnStepArgs;
+
+int kdn_step(const KdnStepArgs* args, kdn_stream_t stream);
+
+/* ------------------------------------------------------------------------ *
+ * The norms around a block: what joins one block's output to the residual
+ * stream and normalises the sum for the next block.
+ *
+ *   u = act(gate) scale norm(y) post_weight,  z = alpha x + u,
+ *   h = norm(z) weight,   norm(t) = t / sqrt(mean(t^2) + eps)
+ *
+ * Rows of D values (1 <= D <= 16384), row-contiguous with the row strides
+ * given (elements).  x, z, dz, dx: bf16 or fp32 (stream_bf16); y, gate, h, dh,
+ * dy, dgate: bf16 or fp32 (act_bf16; an fp32 act_bf16 = 0 needs an fp32
+ * stream).  post_weight NULL: no norm after the block (norm(y) post_weight is
+ * y); gate NULL: act = 1; scale NULL: 1; y NULL: no block (z = x is not
+ * written, alpha must be 1).  act is sigmoid(g) or (swish) g sigmoid(g).
+ * Weights and their gradients: fp32, or bf16 (weights_bf16).
+ *
+ * The forward writes z, h and the statistics rstd [2, rows] fp32 (row 0: of y,
+ * row 1: of z), nullable when no backward follows.  The backward takes the
+ * cotangents dz, dh (either may be NULL: zero; contiguous) and writes dx, dy,
+ * dgate (contiguous) and dweight, dpost, dscale [D] (each nullable when not
+ * needed).  Workspace: kdn_block_norm_workspace_bytes(rows, D), only when a
+ * weight gradient is asked for.  Zero-initialise the struct.
+ * ------------------------------------------------------------------------ */
+typedef struct KdnBlockNormArgs {
+  int32_t stream_bf16, act_bf16, weights_bf16, swish;
+  int64_t rows, D;
+  float alpha, eps;
+  const void* x;
+  const void* y;
+  const void* gate;
+  int64_t x_stride, y_stride, gate_stride;
+  const void* weight;
+  const void* post_weight;
+  const void* scale;
+  void* z;
+  void* h;
+  float* rstd;
+  const void* dz;
+  const void* dh;
+  void* dx;
+  void* dy;
+  void* dgate;
+  void* dweight;
+  void* dpost;
+  void* dscale;
+  void* workspace;
+  size_t workspace_bytes;
+} KdnBlockNormArgs;
+
+size_t kdn_block_norm_workspace_bytes(int64_t rows, int64_t D);
+int kdn_block_norm_fwd(const KdnBlockNormArgs* args, kdn_stream_t stream);
+int kdn_block_norm_bwd(const KdnBlockNormArgs* args, kdn_stream_t stream);
+
+/* ------------------------------------------------------------------------ *
+ * One token per row of logits [rows, V] under temperature, top-k, top-p and
+ * min-p, from given Exp(1) random numbers noise [rows, V].
+ *
+ *   e_i = exp((l_i - max l) / T)  (1 where l_i = max l),  Z = sum e
+ *   order: larger logit first, among equal ones the lower index
+ *   kept: rank < top_k, sum of e over the tokens ahead < top_p Z (no such
+ *         limit for top_p >= 1),
+ *         e >= min_p, e > 0; the first of the order always
+ *   token = the kept token with the largest e_i / noise_i (the lowest rank
+ *           among equal ones), prob = e_token / Z
+ *
+ * so that a kept token is drawn with probability e_i / sum of the kept e.
+ * T <= 0: the first of the order, prob 1.  NaN logits count as -inf; a row
+ * with nothing above -inf gives token -1, prob 0.  top_k <= 0: no limit.
+ * temperature, top_p, min_p: fp32 [rows] or NULL with the value for all rows
+ * beside it; top_k: int32 [rows] (int64 if top_k_i64) or NULL likewise.
+ * logits: bf16 (logits_bf16) or fp32, noise fp32, with row strides (elements).
+ * token: int64 [rows], prob: fp32 [rows].  V < 2^31.  Workspace:
+ * kdn_sample_workspace_bytes(rows, V).  Zero-initialise the struct.
+ * ------------------------------------------------------------------------ */
+typedef struct KdnSampleArgs {
+  int32_t logits_bf16, top_k_i64;
+  int64_t rows, V;
+  const void* logits;
+  const float* noise;
+  int64_t logits_stride, noise_stride;
+  const float* temperature;
+  const void* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int64_t top_k_all;
+  float top_p_all, min_p_all;
+  int64_t* token;
+  float* prob;
+  void* workspace;
+  size_t workspace_bytes;
+} KdnSampleArgs;
+
+size_t kdn_sample_workspace_bytes(int64_t rows, int64_t V);
+int kdn_sample(const KdnSampleArgs* args, kdn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -70,6 +70,46 @@ class KdnScanArgs(ctypes.Structure):
     ]
 
 
+def _struct(name, *groups):
+    """A ctypes structure with the header's fields: (type, "names") groups in order."""
+    fields = [(field, ctype) for ctype, names in groups for field in names.split()]
+    return type(name, (ctypes.Structure,), {"_fields_": fields})
+
+
+KdnStepArgs = _struct(
+    "KdnStepArgs",
+    (ctypes.c_int32, "variant act_bf16 swish slots_i64"),
+    (ctypes.c_int64, "B H D num_slots"),
+    (ctypes.c_void_p, "qkv decay_raw omega_raw r_raw gate"),
+    (ctypes.c_int64, "qkv_stride decay_stride omega_stride r_stride gate_stride"),
+    (ctypes.c_void_p, "conv_weight A_log dt_bias omega_bias r_bias norm_weight"),
+    (ctypes.c_float, "omega_min r_min posterior_scale eps scale"),
+    (ctypes.c_void_p, "slots memory covariance window y"),
+)
+KdnBlockNormArgs = _struct(
+    "KdnBlockNormArgs",
+    (ctypes.c_int32, "stream_bf16 act_bf16 weights_bf16 swish"),
+    (ctypes.c_int64, "rows D"),
+    (ctypes.c_float, "alpha eps"),
+    (ctypes.c_void_p, "x y gate"),
+    (ctypes.c_int64, "x_stride y_stride gate_stride"),
+    (ctypes.c_void_p, "weight post_weight scale z h rstd dz dh dx dy dgate dweight dpost dscale workspace"),
+    (ctypes.c_size_t, "workspace_bytes"),
+)
+KdnSampleArgs = _struct(
+    "KdnSampleArgs",
+    (ctypes.c_int32, "logits_bf16 top_k_i64"),
+    (ctypes.c_int64, "rows V"),
+    (ctypes.c_void_p, "logits noise"),
+    (ctypes.c_int64, "logits_stride noise_stride"),
+    (ctypes.c_void_p, "temperature top_k top_p min_p"),
+    (ctypes.c_float, "temperature_all"),
+    (ctypes.c_int64, "top_k_all"),
+    (ctypes.c_float, "top_p_all min_p_all"),
+    (ctypes.c_void_p, "token prob workspace"),
+    (ctypes.c_size_t, "workspace_bytes"),
+)
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
@@ -139,6 +179,12 @@ _SIGNATURES = {
     "kdn_scan_workspace_bytes": ([ctypes.POINTER(KdnScanArgs)], _SZ),
     "kdn_scan_fwd": ([ctypes.POINTER(KdnScanArgs), _P], ctypes.c_int),
     "kdn_scan_bwd": ([ctypes.POINTER(KdnScanArgs), _P], ctypes.c_int),
+    "kdn_step": ([ctypes.POINTER(KdnStepArgs), _P], ctypes.c_int),
+    "kdn_block_norm_workspace_bytes": ([_I64, _I64], _SZ),
+    "kdn_block_norm_fwd": ([ctypes.POINTER(KdnBlockNormArgs), _P], ctypes.c_int),
+    "kdn_block_norm_bwd": ([ctypes.POINTER(KdnBlockNormArgs), _P], ctypes.c_int),
+    "kdn_sample_workspace_bytes": ([_I64, _I64], _SZ),
+    "kdn_sample": ([ctypes.POINTER(KdnSampleArgs), _P], ctypes.c_int),
 }
 
 
