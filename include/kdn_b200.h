@@ -622,7 +622,7 @@ int kdn_step(const KdnStepArgs* args, kdn_stream_t stream);
  *   u = act(gate) scale norm(y) post_weight,  z = alpha x + u,
  *   h = norm(z) weight,   norm(t) = t / sqrt(mean(t^2) + eps)
  *
- * Rows of D values (1 <= D <= 16384), row-contiguous with the row strides
+ * Rows of D values (2 <= D <= 8192), row-contiguous with the row strides
  * given (elements).  x, z, dz, dx: bf16 or fp32 (stream_bf16); y, gate, h, dh,
  * dy, dgate: bf16 or fp32 (act_bf16; an fp32 act_bf16 = 0 needs an fp32
  * stream).  post_weight NULL: no norm after the block (norm(y) post_weight is

@@ -22,13 +22,14 @@ from torch.autograd.function import once_differentiable
 from . import _native as N
 from .norm_gated import _ACTIVATIONS
 
-MAX_WIDTH = 16384
+# A norm over one value is its sign; its gradient is of the order of eps, which fp32 cannot resolve beside 1.
+MIN_WIDTH, MAX_WIDTH = 2, 8192
 
 
 def _rows(t, D):
     """[..., D] as [rows, D] with contiguous rows (a view where the strides allow one)."""
     t = t.reshape(-1, D)
-    return t if t.stride(1) == 1 or D == 1 else t.contiguous()
+    return t if t.stride(1) == 1 else t.contiguous()
 
 
 def _args(x, y, gate, weight, post_weight, scale, alpha, swish, eps):
@@ -98,6 +99,7 @@ class _BlockNormFunction(torch.autograd.Function):
         grads = []
         for t, needed, name in zip((x, y, gate, weight, post_weight, scale), ctx.needs_input_grad,
                                    ("dx", "dy", "dgate", "dweight", "dpost", "dscale")):
+            needed = needed and not (name == "dweight" and dh is None)  # z does not depend on the weight
             out = torch.empty(t.shape, dtype=t.dtype, device=t.device) if needed else None
             if needed:
                 setattr(a, name, out.data_ptr())
@@ -113,8 +115,8 @@ class _BlockNormFunction(torch.autograd.Function):
 def _validate(x, y, weight, post_weight, gate, scale, alpha, activation):
     if activation not in _ACTIVATIONS:
         raise ValueError(f"Unsupported activation: {activation}")
-    if x.ndim < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
-        raise ValueError(f"kdn_b200 block_norm: the last axis must be 1 to {MAX_WIDTH} wide, got {tuple(x.shape)}")
+    if x.ndim < 1 or not MIN_WIDTH <= x.shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"kdn_b200 block_norm: the last axis must be {MIN_WIDTH} to {MAX_WIDTH} wide, got {tuple(x.shape)}")
     D = x.shape[-1]
     if x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"x must be bf16 or fp32, got {x.dtype}")
