@@ -676,16 +676,18 @@ int kdn_block_norm_bwd(const KdnBlockNormArgs* args, kdn_stream_t stream);
  *   kept: rank < top_k, sum of e over the tokens ahead < top_p Z (no such
  *         limit for top_p >= 1),
  *         e >= min_p, e > 0; the first of the order always
- *   token = the kept token with the largest e_i / noise_i (the lowest rank
- *           among equal ones), prob = e_token / Z
+ *   token = the kept token with the largest e_i / noise_i (the lowest index
+ *           among equal ones; the first of the order if none is positive),
+ *   prob = e_token / Z
  *
  * so that a kept token is drawn with probability e_i / sum of the kept e.
- * T <= 0: the first of the order, prob 1.  NaN logits count as -inf; a row
- * with nothing above -inf gives token -1, prob 0.  top_k <= 0: no limit.
+ * T <= 0: the first of the order, prob 1.  NaN logits count as -inf, +inf
+ * as the largest fp32 value; a row with nothing above -inf gives token -1,
+ * prob 0.  top_k <= 0: no limit.
  * temperature, top_p, min_p: fp32 [rows] or NULL with the value for all rows
  * beside it; top_k: int32 [rows] (int64 if top_k_i64) or NULL likewise.
  * logits: bf16 (logits_bf16) or fp32, noise fp32, with row strides (elements).
- * token: int64 [rows], prob: fp32 [rows].  V < 2^31.  Workspace:
+ * token: int64 [rows], prob: fp32 [rows].  V <= 2^29.  Workspace:
  * kdn_sample_workspace_bytes(rows, V).  Zero-initialise the struct.
  * ------------------------------------------------------------------------ */
 typedef struct KdnSampleArgs {

@@ -8,17 +8,18 @@
 // No sort is needed, because the kept set is a prefix.  A cluster of CTAs
 // holds a row in shared memory (read once) and
 //  1. finds the maximum,
-//  2. sums Z and fills a histogram over 1/16-octave bins of e, whose integer
-//     entries bound the count and the mass ahead of every bin from both sides:
-//     tokens from bin `cut` on are certainly dropped, those before bin `safe`
-//     are certainly within top-k and top-p,
+//  2. sums Z and fills a histogram of e over 1/16 octaves (the bins are the
+//     leading bits of the float e).  A bin's entry is the whole-number sum of
+//     its tokens' mantissas: it bounds their count from both sides and gives
+//     their mass, so that tokens behind `cut` are certainly dropped and those
+//     before `safe` certainly within top-k and top-p,
 //  3. races the tokens before `cut` (only their random numbers are read).  A
 //     winner before `safe` is the answer.  Otherwise the exact count and mass
 //     ahead of it are taken; if it is not kept, the tokens ahead of it race.
 // Every race lost drops the winner and what is behind it; after kRaces of them
 // (noise that follows the logits) the end of the kept prefix is bisected
-// instead, so that no row takes more than kRaces + 64 turns.  Sums have a fixed
-// order or are integers.
+// instead, so that no row takes more than kRaces + 64 turns.  Rows without
+// top-k and top-p race in step 2.  Sums have a fixed order or are integers.
 #include <cooperative_groups.h>
 
 #include "kdn_common.cuh"
@@ -33,30 +34,29 @@ constexpr int kSmChunk = 16384;     // tokens per CTA before a row gets another 
 constexpr int kSmHeld = 192 * 1024;  // bytes of shared memory for them; what a chunk has beyond is read again in every pass
 constexpr int kSmCluster = 8;
 constexpr int kRaces = 12;
-constexpr int kBins = 1024;       // of 1/16 octave: e down to 2^-64
-constexpr float kPerOctave = 16.f;
-constexpr float kBinLow = 0.957f;  // 2^(-1/16), rounded down: the smallest e of a bin over its largest
+constexpr float kLargest = 3.402823466e38f;
+constexpr int kBins = 1024;      // e from 1 down to 2^-64
+constexpr int kBinShift = 23 - 4;  // 16 bins per octave
+constexpr uint32_t kOne = 0x3f800000u;  // the bits of e = 1
 
-struct Best {  // a race's leader: the larger score, then the earlier in the order
+struct Best {  // a race's leader: the larger score, then the lower index; score 0: nobody
   float score, logit;
   int index;
 };
 __device__ __forceinline__ bool ahead(float la, int ia, float lb, int ib) { return la > lb || (la == lb && ia < ib); }
-__device__ __forceinline__ bool beats(const Best& a, const Best& b) {
-  return a.score > b.score || (a.score == b.score && ahead(a.logit, a.index, b.logit, b.index));
+// over the warp's lanes; scores are not negative, so their bits are in order
+__device__ __forceinline__ Best warp_best(const Best& b) {
+  const uint32_t bits = __float_as_uint(b.score), most = __reduce_max_sync(~0u, bits);
+  const uint32_t index = bits == most ? (uint32_t)b.index : ~0u, low = __reduce_min_sync(~0u, index);
+  const int lane = __ffs(__ballot_sync(~0u, index == low)) - 1;
+  return Best{__uint_as_float(most), __shfl_sync(~0u, b.logit, lane), (int)low};
 }
-__device__ __forceinline__ Best shuffle(const Best& b, int o) {
-  return Best{__shfl_xor_sync(~0u, b.score, o), __shfl_xor_sync(~0u, b.logit, o), __shfl_xor_sync(~0u, b.index, o)};
-}
-__device__ __forceinline__ Best warp_best(Best b) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Best c = shuffle(b, o);
-    if (beats(c, b)) b = c;
-  }
-  return b;
-}
-__device__ __forceinline__ float clean(float l) { return isnan(l) ? -INFINITY : l; }
+// What a reduction carries beside it.
+struct Part {
+  Best best;
+  float mass;
+  int count;
+};
 
 // Whole-number keys in the order of the logits.
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -74,6 +74,7 @@ struct Chunk {
   static constexpr int kPer = VEC ? 8 : 1;
   const T* row;
   int begin, end, groups;  // groups of kSmThreads * kPer tokens in shared memory
+  bool infinite = false;    // +inf is among the row's logits: it counts as the largest finite value
   T* held;
 
   __device__ __forceinline__ int first(int j) const { return begin + (j * kSmThreads + (int)threadIdx.x) * kPer; }
@@ -82,7 +83,7 @@ struct Chunk {
     return held + (size_t)(VEC && sizeof(T) == 4 ? 2 * j * kSmThreads * 4 + threadIdx.x * 4
                                                  : (j * kSmThreads + threadIdx.x) * kPer);
   }
-  __device__ __forceinline__ void load() {
+  __device__ __forceinline__ void request() {
 #pragma unroll 4
     for (int j = 0; j < groups; ++j) {
       const int i = first(j);
@@ -103,196 +104,219 @@ struct Chunk {
       }
     }
     cp_async_commit();
-    cp_async_wait_all();
   }
-  // f(logit, index) for this thread's tokens, in a fixed order (past the end: -inf)
+  // f(logits, first index, how many) for this thread's groups, in a fixed order (past the end: -inf)
   template <class F>
   __device__ __forceinline__ void each(F&& f) const {
 #pragma unroll 1
     for (int j = 0; j < groups; ++j) {
-      const int i = first(j);
       const T* at = place(j);
+      float v[kPer];
       if constexpr (!VEC) {
-        f(clean(to_f(*at)), i);
+        v[0] = to_f(*at);
+      } else if constexpr (sizeof(T) == 2) {
+        ld8(v, at);
       } else {
-        float v[8];
-        if constexpr (sizeof(T) == 2) {
-          ld8(v, at);
-        } else {
-          const float4 p = *reinterpret_cast<const float4*>(at), q = *reinterpret_cast<const float4*>(at + kSmThreads * 4);
-          v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f(clean(v[k]), i + k);
+        const float4 p = *reinterpret_cast<const float4*>(at), q = *reinterpret_cast<const float4*>(at + kSmThreads * 4);
+        v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
       }
+      if (infinite)
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) v[k] = fminf(v[k], kLargest);
+      f(v, first(j));
     }
-    for (int i = begin + groups * kSmThreads * kPer + (int)threadIdx.x; i < end; i += kSmThreads) f(clean(to_f(row[i])), i);
+    const int done = groups * kSmThreads * kPer;
+#pragma unroll 1
+    for (int j = 0; begin + done + j * kSmThreads < end; ++j) {
+      const int i = begin + done + j * kSmThreads + (int)threadIdx.x;
+      float v[kPer];
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) v[k] = -INFINITY;
+      if (i < end) v[0] = to_f(row[i]);
+      if (infinite) v[0] = fminf(v[0], kLargest);
+      f(v, i);
+    }
   }
 };
 
 struct Shared {
-  float top[kSmWarps], mass[2][kSmWarps];
-  int first[kSmWarps], count[2][kSmWarps];
-  Best best[2][kSmWarps];
+  Part warps[kSmWarps], ctas[2][kSmCluster];
   uint32_t hist[kBins];
-  unsigned long long scan_s[kSmWarps];
-  float scan_m[kSmWarps];
+  int least[kSmWarps], most[kSmWarps];  // of a scan: the counts' bounds
+  float scan[kSmWarps];
   int cut[kSmWarps], safe[kSmWarps];
 };
 
-// f(value) over the warps' entries of every CTA of the cluster: lane by lane, then `join` over the warp
-template <class V, class J>
-__device__ __forceinline__ V gather(cg::cluster_group& cluster, V* mine, int ctas, V none, J&& join) {
-  const int lane = threadIdx.x & 31;
-  V v = none;
-  for (int e = lane; e < ctas * kSmWarps; e += 32) {
-    V* at = mine + e % kSmWarps;
-    v = join(v, ctas == 1 ? *at : *cluster.map_shared_rank(at, e / kSmWarps));
-  }
-  return v;
+__device__ __forceinline__ Part warp_part(Part p) {
+  p.best = warp_best(p.best);
+  p.mass = warp_sum(p.mass);
+  p.count = __reduce_add_sync(~0u, p.count);
+  return p;
 }
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kSmThreads, 3) sample_kernel(const __grid_constant__ KdnSampleArgs a, int ctas,
-                                                              int chunk, int groups, float fraction) {
+                                                              int chunk, int groups, int down) {
   __shared__ __align__(16) Shared sh;
   extern __shared__ uint4 held[];
   cg::cluster_group cluster = cg::this_cluster();
+  using Tokens = Chunk<T, VEC>;
+  constexpr int PER = Tokens::kPer;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = (int)a.V;
   const int64_t row = blockIdx.x / ctas;
   const int rank = (int)(blockIdx.x % ctas);
-  auto meet = [&] {
-    if (ctas == 1) __syncthreads();
-    else cluster.sync();
+  const Best nobody{0.f, -INFINITY, INT32_MAX};
+  const Part nothing{nobody, 0.f, 0};
+  int buf = 0;
+  // Over all threads of the cluster, in the same order in each of them: lanes,
+  // warps, then CTAs, which write their part into each other's memory.
+  auto reduce = [&](Part p) {
+    p = warp_part(p);
+    if (lane == 0) sh.warps[warp] = p;
+    __syncthreads();
+    if (ctas == 1) {
+      p = warp_part(lane < kSmWarps ? sh.warps[lane] : nothing);
+      __syncthreads();  // the entries may be written again
+      return p;
+    }
+    if (warp == 0) {
+      p = warp_part(lane < kSmWarps ? sh.warps[lane] : nothing);
+      if (lane < ctas) *cluster.map_shared_rank(&sh.ctas[buf][rank], lane) = p;
+    }
+    cluster.sync();
+    p = warp_part(lane < ctas ? sh.ctas[buf][lane] : nothing);
+    buf ^= 1;
+    return p;
   };
-  const float temp = a.temperature ? a.temperature[row] : a.temperature_all;
-  const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
-  int64_t top_k = !a.top_k ? a.top_k_all
-                  : a.top_k_i64 ? static_cast<const int64_t*>(a.top_k)[row]
-                                : (int64_t) static_cast<const int32_t*>(a.top_k)[row];
-  if (top_k <= 0 || top_k > V) top_k = V;
-  const bool greedy = !(temp > 0.f), by_rank = !greedy && (top_k < V || top_p < 1.f);
-  const float* E = a.noise + row * a.noise_stride;
-
-  Chunk<T, VEC> c;
+  Tokens c;
   c.row = static_cast<const T*>(a.logits) + row * a.logits_stride;
-  c.begin = min((int64_t)rank * chunk, (int64_t)V);
-  c.end = min((int64_t)c.begin + chunk, (int64_t)V);
+  c.begin = (int)min((int64_t)rank * chunk, (int64_t)V);
+  c.end = (int)min((int64_t)c.begin + chunk, (int64_t)V);
   c.groups = groups;
   c.held = reinterpret_cast<T*>(held);
-  c.load();
-  if (by_rank)
-    for (int i = tid; i < kBins; i += kSmThreads) sh.hist[i] = 0;
+  c.request();
+  const float temp = a.temperature ? a.temperature[row] : a.temperature_all;
+  const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, min_p = a.min_p ? a.min_p[row] : a.min_p_all;
+  int64_t limit = !a.top_k ? a.top_k_all
+                  : a.top_k_i64 ? static_cast<const int64_t*>(a.top_k)[row]
+                                : (int64_t) static_cast<const int32_t*>(a.top_k)[row];
+  const int top_k = limit <= 0 || limit > V ? V : (int)limit;
+  const bool greedy = !(temp > 0.f), by_rank = !greedy && (top_k < V || top_p < 1.f);
+  const float* E = a.noise + row * a.noise_stride;
+  for (int i = tid; i < kBins; i += kSmThreads) sh.hist[i] = 0;
+  cp_async_wait_all();
 
   // ---- 1: the maximum ----
   float m = -INFINITY;
-  c.each([&](float l, int) { m = fmaxf(m, l); });
-  m = warp_max(m);
-  if (lane == 0) sh.top[warp] = m;
-  meet();
-  const float top = warp_max(gather(cluster, sh.top, ctas, -INFINITY, [](float x, float y) { return fmaxf(x, y); }));
-  if (top == -INFINITY) {
-    if (rank == 0 && tid == 0) a.token[row] = -1, a.prob[row] = 0.f;
-    meet();  // nobody leaves while its memory may be read
-    return;
-  }
+  c.each([&](const float (&v)[PER], int) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) m = fmaxf(m, v[k]);  // passes over NaN
+  });
+  // as a race whose scores are the keys (0: no token), read back as their bits
+  float top = logit_of(__float_as_uint(reduce(Part{Best{__uint_as_float(key_of(m)), 0.f, tid}, 0.f, 0}).best.score));
+  c.infinite = top == INFINITY;
+  if (c.infinite) top = kLargest;
 
-  // ---- 2: Z, the order's first token, the histogram or the only race ----
-  // octaves below the maximum, the product kept exact enough by a second term
-  const float scale = 1.4426950408889634f / temp, rest = fmaf(-scale, temp, 1.4426950408889634f) / temp;
-  auto octaves = [&](float l) {
-    const float d = top - l;  // inf or (two infinities) NaN for infinite logits
-    return l == top ? 0.f : d < INFINITY ? fmaf(d, scale, d * rest) : INFINITY;
+  // ---- 2: Z, and the histogram or the only race ----
+  // e = 2^-t, t = (top - l) log2(e) / T in two terms; both are positive, so that -inf gives t = inf, e = 0
+  const float scale = __fdiv_rd(1.4426950408889634f, temp);
+  const float rest = fmaxf(fmaf(-scale, temp, 1.4426950408889634f) / temp, 1e-30f);
+  auto weight = [&](float l) { return fmaxf(ex2a(-fmaf(top - l, scale, (top - l) * rest)), 0.f); };  // NaN: 0
+  Best best = nobody;
+  auto enter = [&](float e, float noise, float l, int i) {  // a thread's indexes grow: ties stay with the first
+    const float score = __fdividef(e, noise);
+    if (score > best.score) best = Best{score, l, i};
   };
-  auto score = [&](float e, int i) { return __fdividef(e, E[i]); };
-  float z = 0.f;
-  int first = INT32_MAX;
-  Best best{-1.f, -INFINITY, INT32_MAX};
-  auto enter = [&](float e, float l, int i) {
-    const Best b{score(e, i), l, i};
-    if (beats(b, best)) best = b;
-  };
-  if (greedy) {
-    c.each([&](float l, int i) {
-      if (l == top) first = min(first, i);
-    });
-  } else {
-    c.each([&](float l, int i) {
-      if (l == top) first = min(first, i);
-      const float t = octaves(l), e = ex2a(-t);
-      z += e;
+  float Z = 0.f;
+  if (!greedy && top > -INFINITY) {
+    const bool noise16 = VEC && ((reinterpret_cast<uintptr_t>(E) & 15) == 0);
+    c.each([&](const float (&v)[PER], int i) {
+      float e[PER];
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        e[k] = weight(v[k]);
+        Z += e[k];
+      }
       if (by_rank) {
-        const float bin = floorf(t * kPerOctave);
-        if (bin < (float)kBins)
-          atomicAdd(&sh.hist[(int)bin], (uint32_t)(ex2a(bin * (1.f / kPerOctave) - t) * fraction));
-      } else if (e > 0.f && e >= min_p) {
-        enter(e, l, i);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const uint32_t u = __float_as_uint(e[k]) - 1, bin = (kOne - 1 - u) >> kBinShift;
+          if (bin < kBins) atomicAdd(&sh.hist[bin], ((u & 0x7fffffu) | 0x800000u) >> (8 + down));
+        }
+      } else {
+        float noise[PER];
+        if (PER == 8 && noise16 && i + 8 <= c.end) {
+          const float4 p = __ldg(reinterpret_cast<const float4*>(E + i)), q = __ldg(reinterpret_cast<const float4*>(E + i + 4));
+          noise[0] = p.x; noise[1 % PER] = p.y; noise[2 % PER] = p.z; noise[3 % PER] = p.w;
+          noise[4 % PER] = q.x; noise[5 % PER] = q.y; noise[6 % PER] = q.z; noise[7 % PER] = q.w;
+        } else {
+#pragma unroll
+          for (int k = 0; k < PER; ++k) noise[k] = i + k < c.end ? E[i + k] : 1.f;
+        }
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+          if (e[k] >= min_p) enter(e[k], noise[k], v[k], i + k);
       }
     });
   }
-  z = warp_sum(z);
-  first = __reduce_min_sync(~0u, first);
-  best = warp_best(best);
-  if (lane == 0) sh.mass[0][warp] = z, sh.first[warp] = first, sh.best[0][warp] = best;
-  meet();
-  // the CTAs' sums one after the other: the same order in every thread
-  const float Z = warp_sum(gather(cluster, sh.mass[0], ctas, 0.f, [](float x, float y) { return x + y; }));
-  first = __reduce_min_sync(~0u, gather(cluster, sh.first, ctas, INT32_MAX, [](int x, int y) { return min(x, y); }));
-  auto faster = [](const Best& x, const Best& y) { return beats(y, x) ? y : x; };
-  const Best nobody{-1.f, -INFINITY, INT32_MAX};
-  Best win = greedy ? nobody : warp_best(gather(cluster, sh.best[0], ctas, nobody, faster));
+  const Part second = reduce(Part{best, Z, 0});
+  Z = second.mass;
+  Best win = second.best;
 
   // ---- 3: races among the tokens before `cut` ----
-  if (by_rank) {
-    // bins 2 tid and 2 tid + 1 over the cluster
-    unsigned long long s[2] = {0, 0};
-    for (int r = 0; r < ctas; ++r) {
-      const uint2 u = *reinterpret_cast<const uint2*>((ctas == 1 ? sh.hist : cluster.map_shared_rank(sh.hist, r)) + 2 * tid);
-      s[0] += u.x;
-      s[1] += u.y;
+  if (by_rank && top > -INFINITY) {
+    // this thread's two bins over the cluster: bounds of their counts, their mass
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < kSmCluster; ++r)
+      if (r < ctas) {
+        const uint2 u = *reinterpret_cast<const uint2*>((ctas == 1 ? sh.hist : cluster.map_shared_rank(sh.hist, r)) + 2 * tid);
+        sum[0] += (float)u.x;
+        sum[1] += (float)u.y;
+      }
+    int least[2], most[2];
+    float mass[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {  // 1e-6 covers the roundings of sum and quotient
+      const uint32_t u = kOne - 1 - ((uint32_t)(2 * tid + b) << kBinShift);  // the largest of the bin
+      const uint32_t high = ((u & 0x7fffffu) | 0x800000u) >> (8 + down), low = (high + 1) - (1u << (kBinShift - 8 - down));
+      least[b] = (int)ceilf(__fdividef(sum[b], (float)high) * (1.f - 1e-6f));
+      most[b] = (int)(__fdividef(sum[b], (float)low) * (1.f + 1e-6f));
+      mass[b] = sum[b] * __uint_as_float(((u >> 23) - 15 + down) << 23);  // units of 2^(exponent - 15 + down)
     }
-    const float unit = 1.f / fraction;
-    const float mass0 = (float)s[0] * unit * ex2a(-(float)(2 * tid) * (1.f / kPerOctave));
-    const float mass1 = (float)s[1] * unit * ex2a(-(float)(2 * tid + 1) * (1.f / kPerOctave));
-    unsigned long long ps = s[0] + s[1];  // inclusive scans over the threads
-    float pm = mass0 + mass1;
+    int pl_ = least[0] + least[1], pm_ = most[0] + most[1];  // inclusive scans over the threads
+    float ps_ = mass[0] + mass[1];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long us = __shfl_up_sync(~0u, ps, o);
-      const float um = __shfl_up_sync(~0u, pm, o);
-      if (lane >= o) ps += us, pm += um;
+      const int x = __shfl_up_sync(~0u, pl_, o), y = __shfl_up_sync(~0u, pm_, o);
+      const float f = __shfl_up_sync(~0u, ps_, o);
+      if (lane >= o) pl_ += x, pm_ += y, ps_ += f;
     }
-    if (lane == 31) sh.scan_s[warp] = ps, sh.scan_m[warp] = pm;
+    if (lane == 31) sh.least[warp] = pl_, sh.most[warp] = pm_, sh.scan[warp] = ps_;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) ps += sh.scan_s[w], pm += sh.scan_m[w];
-    // before this thread's bins (a lower bound of what is ahead of them), after the first, after the second.
-    // Entries are rounded down by less than one in 0.95 `fraction`; 1e-5 covers the sums' own rounding.
-    const double k_units = (double)top_k * fraction;
-    const float goal = top_p < 1.f ? top_p * Z : INFINITY;
-    int cut = kBins + 1, safe = 0;
-    const float over = 1.f + 2.f / (kBinLow * fraction) + 1e-5f;
-#pragma unroll
-    for (int b = 1; b >= 0; --b) {
-      const unsigned long long sb = b ? ps - s[1] : ps - s[1] - s[0];
-      const float mb = b ? pm - mass1 : pm - mass1 - mass0;
-      if ((double)sb >= k_units || mb * (1.f - 1e-5f) >= goal) cut = 2 * tid + b;
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const unsigned long long sb = b ? ps : ps - s[1];
-      const float mb = b ? pm : pm - mass1;
-      if ((double)sb <= 0.95 * k_units && mb * over < goal) safe = 2 * tid + b + 1;
-    }
+    const bool before = lane < warp;  // warps in front (lane < 16)
+    pl_ += __reduce_add_sync(~0u, before ? sh.least[lane] : 0);
+    pm_ += __reduce_add_sync(~0u, before ? sh.most[lane] : 0);
+    ps_ += warp_sum(before ? sh.scan[lane] : 0.f);
+    // Entries are rounded down by less than one in 2^15 >> down; 1e-5 covers the sums' own rounding.
+    const float goal = top_p < 1.f ? top_p * Z : INFINITY, over = 1.f + (float)(1 << down) / 16384.f + 1e-5f;
+    int cut = kBins, safe = 0;
+    // least and mass ahead of the thread's first and second bin; most and mass up to and with them
+    if (pl_ - least[1] >= top_k || (ps_ - mass[1]) * (1.f - 1e-5f) >= goal) cut = 2 * tid + 1;
+    if (pl_ - least[1] - least[0] >= top_k || (ps_ - mass[1] - mass[0]) * (1.f - 1e-5f) >= goal) cut = 2 * tid;
+    if (pm_ - most[1] <= top_k && (ps_ - mass[1]) * over < goal) safe = 2 * tid + 1;
+    if (pm_ <= top_k && ps_ * over < goal) safe = 2 * tid + 2;
     cut = __reduce_min_sync(~0u, cut);
     safe = __reduce_max_sync(~0u, safe);
     if (lane == 0) sh.cut[warp] = cut, sh.safe[warp] = safe;
     __syncthreads();
     cut = __reduce_min_sync(~0u, sh.cut[lane % kSmWarps]);
     safe = __reduce_max_sync(~0u, sh.safe[lane % kSmWarps]);
-    const float cut_t = cut > kBins ? INFINITY : (float)cut, safe_t = fminf((float)safe, cut_t);
+    // tokens of bins before b have e above these
+    const float e_cut = cut == kBins ? 0.f : __uint_as_float(kOne - ((uint32_t)cut << kBinShift));
+    const float e_safe = fmaxf(__uint_as_float(kOne - ((uint32_t)safe << kBinShift)), e_cut);
 
     // What a turn looks at lies ahead of (pl, pi) in the order.
-    const Best leader{0.f, top, first};
     float pl = -INFINITY;
     int pi = INT32_MAX;
     // bisection: the last kept logit is in [lo, hi] (keys), then the last kept index of it
@@ -300,32 +324,33 @@ __global__ void __launch_bounds__(kSmThreads, 3) sample_kernel(const __grid_cons
     uint32_t lo = 0, hi = 0;
     for (int turn = 0;; ++turn) {
       best = nobody;
-      float mass = 0.f;
+      float weights = 0.f;
       int count = 0;
-      c.each([&](float l, int i) {
-        if (!ahead(l, i, pl, pi)) return;
-        const float t = octaves(l);
-        if (!(t * kPerOctave < cut_t)) return;
-        const float e = ex2a(-t);
-        mass += e;
-        ++count;
-        if (e > 0.f && e >= min_p) enter(e, l, i);
+      c.each([&](const float (&v)[PER], int i) {
+        float most_l = v[0];
+#pragma unroll
+        for (int k = 1; k < PER; ++k) most_l = fmaxf(most_l, v[k]);
+        if (most_l < pl || !(weight(most_l) > e_cut)) return;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const float l = v[k], e = weight(l);
+          if (ahead(l, i + k, pl, pi) && e > e_cut) {
+            weights += e;
+            ++count;
+            if (e >= min_p) enter(e, E[i + k], l, i + k);
+          }
+        }
       });
-      mass = warp_sum(mass);
-      count = __reduce_add_sync(~0u, count);
-      best = warp_best(best);
-      const int buf = 1 - (turn & 1);
-      if (lane == 0) sh.mass[buf][warp] = mass, sh.count[buf][warp] = count, sh.best[buf][warp] = best;
-      meet();
-      mass = warp_sum(gather(cluster, sh.mass[buf], ctas, 0.f, [](float x, float y) { return x + y; }));
-      count = __reduce_add_sync(~0u, gather(cluster, sh.count[buf], ctas, 0, [](int x, int y) { return x + y; }));
-      best = warp_best(gather(cluster, sh.best[buf], ctas, nobody, faster));
+      const Part part = reduce(Part{best, weights, count});
+      best = part.best;
+      weights = part.mass;
+      count = part.count;
       // whether a token at (pl, pi) is within top-k and top-p (the order's first always is)
-      const bool kept = turn > 0 && (count == 0 || (count < top_k && (top_p >= 1.f || mass < top_p * Z)));
+      const bool kept = turn > 0 && (count == 0 || (count < top_k && (top_p >= 1.f || weights < top_p * Z)));
       if (what == kRace) {
         if (kept) break;  // (pl, pi) is the winner
-        win = best.index == INT32_MAX ? leader : best;  // none: no score compares
-        if (win.index == first || octaves(win.logit) * kPerOctave < safe_t) break;
+        win = best;
+        if (win.score == 0.f || weight(win.logit) > e_safe) break;
         if (turn < kRaces) {
           pl = win.logit;
           pi = win.index;
@@ -341,7 +366,7 @@ __global__ void __launch_bounds__(kSmThreads, 3) sample_kernel(const __grid_cons
         if (kept) lo += (hi - lo + 1) / 2;
         else hi = lo + (hi - lo + 1) / 2 - 1;
       } else {
-        win = best.index == INT32_MAX ? leader : best;
+        win = best;
         break;
       }
       if (what == kLogit && lo == hi) {  // every token before the first of this logit is kept
@@ -356,12 +381,23 @@ __global__ void __launch_bounds__(kSmThreads, 3) sample_kernel(const __grid_cons
       if (what == kLast) pi = (int)lo + 1;  // up to and with index lo
     }
   }
-  if (rank == 0 && tid == 0) {
-    if (win.index == INT32_MAX) win = Best{0.f, top, first};  // greedy, or no score compares
-    a.token[row] = win.index;
-    a.prob[row] = greedy ? 1.f : (win.logit == top ? 1.f : expf((win.logit - top) / temp)) / Z;
+
+  // greedy, or nobody's score compares: the order's first token
+  if (win.score == 0.f && top > -INFINITY) {
+    int first = INT32_MAX;
+    c.each([&](const float (&v)[PER], int i) {
+#pragma unroll
+      for (int k = PER - 1; k >= 0; --k)
+        if (v[k] == top) first = min(first, i + k);
+    });
+    win = reduce(Part{Best{first < INT32_MAX ? 1.f : 0.f, top, first}, 0.f, 0}).best;
   }
-  meet();
+  if (rank == 0 && tid == 0) {
+    const bool empty = top == -INFINITY;
+    a.token[row] = empty ? -1 : win.index;
+    a.prob[row] = empty ? 0.f : greedy ? 1.f : expf((win.logit - top) / temp) / Z;
+  }
+  if (ctas > 1) cluster.sync();  // nobody leaves while its memory may be read
 }
 
 template <class T, bool VEC>
@@ -382,8 +418,8 @@ int sample_launch(const KdnSampleArgs& a, cudaStream_t st) {
       return set_error(KDN_ERR_CUDA, "sample_kernel: %s", cudaGetErrorString(err));
     }
   }
-  float fraction = 32768.f;  // units of the histogram: a bin of a CTA's tokens fits 31 bits
-  while (fraction > 1.f && fraction * (float)chunk > 2147483648.f) fraction *= 0.5f;
+  int down = 0;  // a bin's entry, below 2^16 >> down per token, fits 32 bits
+  while ((chunk << 16 >> down) >> 32) ++down;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.rows * ctas));
   cfg.blockDim = dim3(kSmThreads);
@@ -395,7 +431,7 @@ int sample_launch(const KdnSampleArgs& a, cudaStream_t st) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, sample_kernel<T, VEC>, a, (int)ctas, (int)chunk, (int)groups, fraction);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, sample_kernel<T, VEC>, a, (int)ctas, (int)chunk, (int)groups, down);
   if (err != cudaSuccess) {
     cudaGetLastError();
     return set_error(KDN_ERR_CUDA, "sample_kernel: %s", cudaGetErrorString(err));
@@ -419,8 +455,8 @@ size_t kdn_sample_workspace_bytes(int64_t rows, int64_t V) {
 int kdn_sample(const KdnSampleArgs* args, kdn_stream_t stream) {
   if (!args) return set_error(KDN_ERR_INVALID, "kdn_sample: null args");
   const KdnSampleArgs& a = *args;
-  if (a.rows < 0 || a.rows > INT32_MAX / kSmCluster || a.V < 1 || a.V > INT32_MAX - (1 << 16))
-    return set_error(KDN_ERR_INVALID, "kdn_sample: 0 <= rows < 2^28 and 1 <= V < 2^31 - 2^16 required");
+  if (a.rows < 0 || a.rows > INT32_MAX / kSmCluster || a.V < 1 || a.V > (1 << 29))
+    return set_error(KDN_ERR_INVALID, "kdn_sample: 0 <= rows < 2^28 and 1 <= V <= 2^29 required");
   if (a.rows == 0) return KDN_OK;
   if (!a.logits || !a.noise || !a.token || !a.prob) return set_error(KDN_ERR_INVALID, "kdn_sample: null pointer");
   if (a.rows > 1 && (a.logits_stride < a.V || a.noise_stride < a.V))

@@ -4,7 +4,7 @@ given random numbers, in one kernel without a sort.
     e_i = exp((l_i - max l) / T),  Z = sum e          (e = 1 where l is the maximum)
     order: the larger logit first, among equal ones the lower index
     kept:  rank < top_k,  (sum of e ahead) < top_p Z,  e >= min_p;  the first of the order always
-    token = the kept token with the largest e_i / noise_i,  prob = e_token / Z
+    token = the kept token with the largest e_i / noise_i (the lowest index among equal ones),  prob = e_token / Z
 
 Every filter looks at the whole distribution (top-p is not renormalised after
 top-k).  ``noise`` holds independent Exp(1) random numbers
@@ -19,7 +19,7 @@ import torch
 
 from . import _native as N
 
-_VOCAB_LIMIT = 2**31 - 1024
+_VOCAB_LIMIT = 2**29
 
 
 def _option(a, name, value, rows, device, dtypes, cast):
@@ -43,10 +43,10 @@ def sample(logits, noise, *, temperature=1.0, top_k=None, top_p=None, min_p=None
 
     logits [rows, V] bf16 or fp32 and noise [rows, V] fp32 (positive), rows contiguous with any row stride.
     temperature, top_p, min_p: numbers or fp32 tensors [rows]; top_k: int or int32 / int64 tensor [rows]; None,
-    top_k <= 0 or top_p >= 1: no such filter.  temperature <= 0: the most likely token, prob 1.  NaN logits count as -inf; a row with
-    nothing above -inf gives token -1, prob 0.
+    top_k <= 0 or top_p >= 1: no such filter.  temperature <= 0: the most likely token, prob 1.  NaN logits count as -inf and +inf as the
+    largest fp32 value; a row with nothing above -inf gives token -1, prob 0.
     """
-    if logits.ndim != 2 or not 1 <= logits.shape[1] < _VOCAB_LIMIT:
+    if logits.ndim != 2 or not 1 <= logits.shape[1] <= _VOCAB_LIMIT:
         raise ValueError(f"logits must be [rows, V] with V >= 1, got {tuple(logits.shape)}")
     if logits.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"logits must be bf16 or fp32, got {logits.dtype}")
