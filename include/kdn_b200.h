@@ -580,8 +580,8 @@ int kdn_scan_bwd(const KdnScanArgs* args, kdn_stream_t stream);
  * output is zero and no state is touched.  A slot may appear once per call.
  * D = head channels (K = V), 64 or 128.  Activations (qkv, decay_raw,
  * omega_raw, r_raw, gate, window, y) are bf16 (act_bf16 = 1) or fp32; their
- * rows are contiguous, with the row strides given (elements); parameters and
- * states are fp32.  memory and conv_weight must be 16-byte aligned.
+ * rows are contiguous, with the row strides given (elements; 0: one row for
+ * all); parameters and states are fp32.  memory and conv_weight must be 16-byte aligned.
  * Zero-initialise the struct.
  * ------------------------------------------------------------------------ */
 typedef struct KdnStepArgs {
@@ -623,7 +623,7 @@ int kdn_step(const KdnStepArgs* args, kdn_stream_t stream);
  *   h = norm(z) weight,   norm(t) = t / sqrt(mean(t^2) + eps)
  *
  * Rows of D values (2 <= D <= 8192), row-contiguous with the row strides
- * given (elements).  x, z, dz, dx: bf16 or fp32 (stream_bf16); y, gate, h, dh,
+ * given (elements; 0: one row for all).  x, z, dz, dx: bf16 or fp32 (stream_bf16); y, gate, h, dh,
  * dy, dgate: bf16 or fp32 (act_bf16; an fp32 act_bf16 = 0 needs an fp32
  * stream).  post_weight NULL: no norm after the block (norm(y) post_weight is
  * y); gate NULL: act = 1; scale NULL: 1; y NULL: no block (z = x is not
@@ -686,7 +686,8 @@ int kdn_block_norm_bwd(const KdnBlockNormArgs* args, kdn_stream_t stream);
  * prob 0.  top_k <= 0: no limit.
  * temperature, top_p, min_p: fp32 [rows] or NULL with the value for all rows
  * beside it; top_k: int32 [rows] (int64 if top_k_i64) or NULL likewise.
- * logits: bf16 (logits_bf16) or fp32, noise fp32, with row strides (elements).
+ * logits: bf16 (logits_bf16) or fp32, noise fp32, with row strides (elements; 0:
+ * one row for all).
  * token: int64 [rows], prob: fp32 [rows].  V <= 2^29.  Workspace:
  * kdn_sample_workspace_bytes(rows, V).  Zero-initialise the struct.
  * ------------------------------------------------------------------------ */

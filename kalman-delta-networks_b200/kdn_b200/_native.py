@@ -236,6 +236,20 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def launch(entry, args, t: torch.Tensor, what: str) -> None:
+    """Call a C entry ``entry(args, stream)`` on t's current stream, with t's device current."""
+    device = t.device
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return check(entry(args, stream_of(t)), what)
+    check(entry(args, _raw_stream(device.index)), what)
+
+
+def _raw_stream(index: int) -> int:
+    """The handle of the device's current stream (what ``stream_of`` gives, without making a Stream object per call)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 _PRECISION = {"bf16": KDN_PREC_BF16, "fp32": KDN_PREC_FP32}
 
 

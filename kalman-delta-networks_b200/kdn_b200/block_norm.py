@@ -24,11 +24,14 @@ from .norm_gated import _ACTIVATIONS
 
 # A norm over one value is its sign; its gradient is of the order of eps, which fp32 cannot resolve beside 1.
 MIN_WIDTH, MAX_WIDTH = 2, 8192
+_DTYPES = (torch.bfloat16, torch.float32)
 
 
 def _rows(t, D):
-    """[..., D] as [rows, D] with contiguous rows (a view where the strides allow one)."""
-    t = t.reshape(-1, D)
+    """[..., D] as [rows, D] with contiguous rows (a view where the strides allow one).  ``empty_like`` of it is
+    contiguous, whatever the rows' stride."""
+    if t.ndim != 2:
+        t = t.reshape(-1, D)
     return t if t.stride(1) == 1 else t.contiguous()
 
 
@@ -55,19 +58,17 @@ def _forward(x, y, gate, weight, post_weight, scale, alpha, swish, eps, want_rst
     """x, y, gate as [rows, D].  Returns (z or None, h, rstd or None), contiguous."""
     lib = N.load_library()
     a = _args(x, y, gate, weight, post_weight, scale, alpha, swish, eps)
-    rows, D = x.shape
     z = None
     if y is not None:
-        z = torch.empty((rows, D), dtype=x.dtype, device=x.device)
+        z = torch.empty_like(x)
         a.z = z.data_ptr()
-    h = torch.empty((rows, D), dtype=x.dtype if y is None else y.dtype, device=x.device)
+    h = torch.empty_like(x if y is None else y)
     a.h = h.data_ptr()
     rstd = None
     if want_rstd:
-        rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        rstd = x.new_empty((2, x.shape[0]), dtype=torch.float32)
         a.rstd = rstd.data_ptr()
-    with torch.cuda.device(x.device):
-        N.check(lib.kdn_block_norm_fwd(a, N.stream_of(x)), "kdn_block_norm_fwd")
+    N.launch(lib.kdn_block_norm_fwd, a, x, "kdn_block_norm_fwd")
     return z, h, rstd
 
 
@@ -100,15 +101,14 @@ class _BlockNormFunction(torch.autograd.Function):
         for t, needed, name in zip((x, y, gate, weight, post_weight, scale), ctx.needs_input_grad,
                                    ("dx", "dy", "dgate", "dweight", "dpost", "dscale")):
             needed = needed and not (name == "dweight" and dh is None)  # z does not depend on the weight
-            out = torch.empty(t.shape, dtype=t.dtype, device=t.device) if needed else None
+            out = torch.empty_like(t) if needed else None
             if needed:
                 setattr(a, name, out.data_ptr())
             grads.append(out)
         if any(g is not None for g in grads[3:]):
-            ws = N.byte_buffer(lib.kdn_block_norm_workspace_bytes(a.rows, a.D), x.device)
+            ws = x.new_empty(lib.kdn_block_norm_workspace_bytes(a.rows, a.D), dtype=torch.uint8)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        with torch.cuda.device(x.device):
-            N.check(lib.kdn_block_norm_bwd(a, N.stream_of(x)), "kdn_block_norm_bwd")
+        N.launch(lib.kdn_block_norm_bwd, a, x, "kdn_block_norm_bwd")
         return (*grads, None, None, None)
 
 
@@ -118,7 +118,7 @@ def _validate(x, y, weight, post_weight, gate, scale, alpha, activation):
     if x.ndim < 1 or not MIN_WIDTH <= x.shape[-1] <= MAX_WIDTH:
         raise ValueError(f"kdn_b200 block_norm: the last axis must be {MIN_WIDTH} to {MAX_WIDTH} wide, got {tuple(x.shape)}")
     D = x.shape[-1]
-    if x.dtype not in (torch.bfloat16, torch.float32):
+    if x.dtype not in _DTYPES:
         raise TypeError(f"x must be bf16 or fp32, got {x.dtype}")
     if y is None:
         if post_weight is not None or gate is not None or scale is not None or alpha != 1.0:
@@ -130,20 +130,21 @@ def _validate(x, y, weight, post_weight, gate, scale, alpha, activation):
             raise TypeError(f"y must have x's dtype, or be bf16 beside an fp32 x; got x {x.dtype}, y {y.dtype}")
     if gate is not None and (gate.shape != y.shape or gate.dtype != y.dtype):
         raise ValueError(f"gate must have y's shape and dtype, got {tuple(gate.shape)} {gate.dtype}")
+    if weight is None:
+        raise TypeError("weight must be a tensor")
     for name, w in (("weight", weight), ("post_weight", post_weight), ("scale", scale)):
         if w is None:
-            if name == "weight":
-                raise TypeError("weight must be a tensor")
             continue
-        if w.shape != (D,):
+        if w.ndim != 1 or w.shape[0] != D:
             raise ValueError(f"{name} must have shape [{D}], got {tuple(w.shape)}")
-        if w.dtype != weight.dtype or w.dtype not in (torch.bfloat16, torch.float32):
+        if w.dtype is not weight.dtype or w.dtype not in _DTYPES:
             raise TypeError("weight, post_weight and scale must share one dtype, bf16 or fp32")
     device = x.device
     for t in (y, weight, post_weight, gate, scale):
         if t is not None and t.device != device:
             raise ValueError("all block_norm tensors must share one CUDA device")
-    N.require_cuda(x)
+    if not x.is_cuda:
+        N.require_cuda(x)
     return D
 
 
@@ -162,15 +163,19 @@ def block_norm(x, y, weight, *, post_weight=None, gate=None, scale=None, alpha=1
     x2 = _rows(x, D)
     y2 = None if y is None else _rows(y, D)
     g2 = None if gate is None else _rows(gate, D)
-    weight, post_weight, scale = (None if w is None else w.contiguous() for w in (weight, post_weight, scale))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, gate, weight, post_weight,
-                                                                                 scale)):
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad
+                                        for t in (x, y, gate, weight, post_weight, scale)]):
+        weight, post_weight, scale = [None if w is None else w.contiguous() for w in (weight, post_weight, scale)]
         z, h = _BlockNormFunction.apply(x2, y2, g2, weight, post_weight, scale, alpha, swish, eps)
         if y is None and not x.requires_grad:
             z = None
     else:
+        weight, post_weight, scale = [None if w is None else w.contiguous()
+                                      for w in (weight, post_weight, scale)]
         z, h, _ = _forward(x2, y2, g2, weight, post_weight, scale, alpha, swish, eps, False)
-    return (x if z is None else z.view(shape)), h.view(shape)
+    if len(shape) != 2:
+        z, h = None if z is None else z.view(shape), h.view(shape)
+    return (x if z is None else z), h
 
 
 class BlockNorm(nn.Module):

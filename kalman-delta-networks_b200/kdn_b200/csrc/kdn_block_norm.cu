@@ -144,7 +144,8 @@ int block_norm_check(const char* what, const KdnBlockNormArgs* p) {
   if (!a.x || !a.weight) return set_error(KDN_ERR_INVALID, "%s: null pointer", what);
   if (!a.y && (a.gate || a.post_weight || a.scale || a.alpha != 1.f))
     return set_error(KDN_ERR_INVALID, "%s: gate, post_weight, scale and alpha need a block output y", what);
-  if (a.rows > 1 && (a.x_stride < a.D || (a.y && a.y_stride < a.D) || (a.gate && a.gate_stride < a.D)))
+  auto bad = [&](int64_t stride) { return stride < a.D && stride != 0; };  // 0: one row for all
+  if (a.rows > 1 && (bad(a.x_stride) || (a.y && bad(a.y_stride)) || (a.gate && bad(a.gate_stride))))
     return set_error(KDN_ERR_INVALID, "%s: row strides smaller than the rows", what);
   return KDN_OK;
 }

@@ -459,7 +459,8 @@ int kdn_sample(const KdnSampleArgs* args, kdn_stream_t stream) {
     return set_error(KDN_ERR_INVALID, "kdn_sample: 0 <= rows < 2^28 and 1 <= V <= 2^29 required");
   if (a.rows == 0) return KDN_OK;
   if (!a.logits || !a.noise || !a.token || !a.prob) return set_error(KDN_ERR_INVALID, "kdn_sample: null pointer");
-  if (a.rows > 1 && (a.logits_stride < a.V || a.noise_stride < a.V))
+  auto bad = [&](int64_t stride) { return stride < a.V && stride != 0; };  // 0: one row for all
+  if (a.rows > 1 && (bad(a.logits_stride) || bad(a.noise_stride)))
     return set_error(KDN_ERR_INVALID, "kdn_sample: row strides smaller than the rows");
   const int64_t elem = a.logits_bf16 ? 2 : 4;
   const bool vec = ((reinterpret_cast<uintptr_t>(a.logits) | (uintptr_t)(a.rows > 1 ? a.logits_stride * elem : 0)) & 15) == 0;

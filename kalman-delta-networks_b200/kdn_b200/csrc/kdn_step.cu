@@ -245,8 +245,9 @@ extern "C" int kdn_step(const KdnStepArgs* args, kdn_stream_t stream) {
     return set_error(KDN_ERR_INVALID, "kdn_step: size too large");
   const int64_t HD = a.H * a.D;
   const bool diag = a.variant == KDN_DIAG;
-  if (a.B > 1 && (a.qkv_stride < 3 * HD || a.decay_stride < HD || a.gate_stride < HD ||
-                  a.omega_stride < (diag ? HD : a.H) || a.r_stride < a.H))
+  auto bad = [](int64_t stride, int64_t width) { return stride < width && stride != 0; };  // 0: one row for all
+  if (a.B > 1 && (bad(a.qkv_stride, 3 * HD) || bad(a.decay_stride, HD) || bad(a.gate_stride, HD) ||
+                  bad(a.omega_stride, diag ? HD : a.H) || bad(a.r_stride, a.H)))
     return set_error(KDN_ERR_INVALID, "kdn_step: row strides smaller than the rows");
   if (a.B == 0) return KDN_OK;
   if (!a.qkv || !a.decay_raw || !a.omega_raw || !a.r_raw || !a.gate || !a.conv_weight || !a.A_log || !a.dt_bias ||

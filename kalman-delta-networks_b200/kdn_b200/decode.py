@@ -162,8 +162,8 @@ class _Step:
         a.scale = D ** -0.5
         self._args = bytes(a)
 
-    def _run(self, state, slots, qkv, decay_raw, omega_raw, r_raw, out_gate, omega_width):
-        """Checks the token's tensors and launches; omega_raw and r_raw are [B, omega_width] and [B, H]."""
+    def _run(self, state, slots, qkv, rows):
+        """Checks the token's tensors, launches and returns y.  rows: (argument, tensor, width) of those beside qkv."""
         H, channels, dtype = self.num_heads, self.num_heads * self.head_dim, qkv.dtype
         if not isinstance(state, KDNState) or state.variant != self.variant:
             raise TypeError(f"state must be a KDNState of the {self.variant} variant")
@@ -174,45 +174,42 @@ class _Step:
         B, device = qkv.shape[0], qkv.device
         if dtype not in _ACT_DTYPES or dtype != state.window.dtype:
             raise TypeError(f"qkv must be bf16 or fp32 as the state's window ({state.window.dtype}), got {dtype}")
-        for name, t, width in (("decay_raw", decay_raw, channels), ("omega_raw", omega_raw, omega_width),
-                               ("r_raw", r_raw, H), ("out_gate", out_gate, channels)):
-            if t.shape != (B, width):
+        if qkv.stride(1) != 1:
+            raise ValueError(f"qkv's rows must be contiguous, got strides {qkv.stride()}")
+        for name, t, width in rows:
+            if t.ndim != 2 or t.shape[0] != B or t.shape[1] != width:
                 raise ValueError(f"{name} must be {(B, width)}, got {tuple(t.shape)}")
-            if t.dtype != dtype:
+            if t.dtype is not dtype:
                 raise TypeError(f"{name} must have qkv's dtype {dtype}, got {t.dtype}")
-            if t.stride(1) != 1:
+            if t.stride(1) != 1 and width > 1:
                 raise ValueError(f"{name}'s rows must be contiguous, got strides {t.stride()}")
             if t.device != device:
                 raise ValueError("all step tensors must share one CUDA device")
-        if qkv.stride(1) != 1:
-            raise ValueError(f"qkv's rows must be contiguous, got strides {qkv.stride()}")
         if slots is None:
             if state.num_slots < B:
                 raise ValueError(f"without slots the pool must hold {B} states, got {state.num_slots}")
         else:
-            if slots.shape != (B,) or slots.dtype not in _SLOT_DTYPES or not slots.is_contiguous():
+            if slots.ndim != 1 or slots.shape[0] != B or slots.dtype not in _SLOT_DTYPES or not slots.is_contiguous():
                 raise ValueError(f"slots must be a contiguous int32 or int64 [{B}] tensor, got {tuple(slots.shape)} "
                                  f"{slots.dtype}")
             if slots.device != device:
                 raise ValueError("all step tensors must share one CUDA device")
         if state.memory.device != device or self.device != device:
             raise ValueError("all step tensors must share one CUDA device")
-        N.require_cuda(qkv)
+        if not qkv.is_cuda:
+            N.require_cuda(qkv)
         lib = N.load_library()
-        y = torch.empty((B, channels), dtype=dtype, device=device)
+        y = qkv.new_empty((B, channels))
         a = N.KdnStepArgs.from_buffer_copy(self._args)
         a.act_bf16 = dtype == torch.bfloat16
         a.B, a.num_slots = B, state.num_slots
-        a.qkv, a.decay_raw, a.omega_raw = qkv.data_ptr(), decay_raw.data_ptr(), omega_raw.data_ptr()
-        a.r_raw, a.gate = r_raw.data_ptr(), out_gate.data_ptr()
-        a.qkv_stride, a.decay_stride, a.omega_stride = qkv.stride(0), decay_raw.stride(0), omega_raw.stride(0)
-        a.r_stride, a.gate_stride = r_raw.stride(0), out_gate.stride(0)
+        a.qkv, a.qkv_stride = qkv.data_ptr(), qkv.stride(0)
+        self._rows(a, *(t for _, t, _ in rows))
         if slots is not None:
             a.slots, a.slots_i64 = slots.data_ptr(), slots.dtype == torch.int64
         a.memory, a.covariance = state.memory.data_ptr(), state.covariance.data_ptr()
         a.window, a.y = state.window.data_ptr(), y.data_ptr()
-        with torch.cuda.device(device):
-            N.check(lib.kdn_step(a, N.stream_of(qkv)), "kdn_step")
+        N.launch(lib.kdn_step, a, qkv, "kdn_step")
         return y
 
 
@@ -244,9 +241,16 @@ class IsoKDNStep(_Step):
         (None: row b uses slot b; a slot outside the pool marks an idle row, output zero; no slot twice).
         Returns y [B, H*D] and updates the states in place."""
         H = self.num_heads
-        if omega_r_raw.ndim != 2 or omega_r_raw.shape[1] != 2 * H:
-            raise ValueError(f"omega_r_raw must be [B, {2 * H}], got {tuple(omega_r_raw.shape)}")
-        return self._run(state, slots, qkv, decay_raw, omega_r_raw[:, :H], omega_r_raw[:, H:], out_gate, H)
+        channels = H * self.head_dim
+        return self._run(state, slots, qkv, (("decay_raw", decay_raw, channels), ("omega_r_raw", omega_r_raw, 2 * H),
+                                             ("out_gate", out_gate, channels)))
+
+    def _rows(self, a, decay_raw, omega_r_raw, out_gate):
+        a.decay_raw, a.decay_stride = decay_raw.data_ptr(), decay_raw.stride(0)
+        a.omega_raw, a.omega_stride = omega_r_raw.data_ptr(), omega_r_raw.stride(0)
+        a.r_raw = omega_r_raw.data_ptr() + self.num_heads * omega_r_raw.element_size()  # the row's second half
+        a.r_stride = omega_r_raw.stride(0)
+        a.gate, a.gate_stride = out_gate.data_ptr(), out_gate.stride(0)
 
 
 class DiagKDNStep(_Step):
@@ -262,8 +266,16 @@ class DiagKDNStep(_Step):
 
     def __call__(self, state, qkv, retention_raw, omega_raw, r_raw, out_gate, slots=None):
         """As :meth:`IsoKDNStep.__call__`, with retention_raw and omega_raw [B, H*D] and r_raw [B, H]."""
-        return self._run(state, slots, qkv, retention_raw, omega_raw, r_raw, out_gate,
-                         self.num_heads * self.head_dim)
+        channels = self.num_heads * self.head_dim
+        return self._run(state, slots, qkv, (("retention_raw", retention_raw, channels),
+                                             ("omega_raw", omega_raw, channels), ("r_raw", r_raw, self.num_heads),
+                                             ("out_gate", out_gate, channels)))
+
+    def _rows(self, a, retention_raw, omega_raw, r_raw, out_gate):
+        a.decay_raw, a.decay_stride = retention_raw.data_ptr(), retention_raw.stride(0)
+        a.omega_raw, a.omega_stride = omega_raw.data_ptr(), omega_raw.stride(0)
+        a.r_raw, a.r_stride = r_raw.data_ptr(), r_raw.stride(0)
+        a.gate, a.gate_stride = out_gate.data_ptr(), out_gate.stride(0)
 
 
 __all__ = ("KDNState", "IsoKDNStep", "DiagKDNStep")

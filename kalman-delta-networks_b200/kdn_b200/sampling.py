@@ -30,7 +30,7 @@ def _option(a, name, value, rows, device, dtypes, cast):
         except (TypeError, ValueError):
             raise TypeError(f"{name} must be a number, a tensor [{rows}] or None, got {value!r}") from None
         return
-    if value.shape != (rows,) or value.dtype not in dtypes or not value.is_contiguous():
+    if value.ndim != 1 or value.shape[0] != rows or value.dtype not in dtypes or not value.is_contiguous():
         raise ValueError(f"{name} must be a contiguous [{rows}] tensor of {' or '.join(map(str, dtypes))}, got "
                          f"{tuple(value.shape)} {value.dtype}")
     if value.device != device:
@@ -64,17 +64,17 @@ def sample(logits, noise, *, temperature=1.0, top_k=None, top_p=None, min_p=None
     _option(a, "top_k", 0 if top_k is None else top_k, rows, device, (torch.int32, torch.int64), int)
     _option(a, "top_p", 1.0 if top_p is None else top_p, rows, device, (torch.float32,), float)
     _option(a, "min_p", 0.0 if min_p is None else min_p, rows, device, (torch.float32,), float)
-    N.require_cuda(logits)
+    if not logits.is_cuda:
+        N.require_cuda(logits)
     lib = N.load_library()
     a.logits_bf16 = logits.dtype == torch.bfloat16
     a.top_k_i64 = isinstance(top_k, torch.Tensor) and top_k.dtype == torch.int64
     a.logits, a.noise = logits.data_ptr(), noise.data_ptr()
     a.logits_stride, a.noise_stride = logits.stride(0), noise.stride(0)
-    token = torch.empty(rows, dtype=torch.int64, device=device)
-    prob = torch.empty(rows, dtype=torch.float32, device=device)
+    token = noise.new_empty(rows, dtype=torch.int64)
+    prob = noise.new_empty(rows)
     a.token, a.prob = token.data_ptr(), prob.data_ptr()
-    with torch.cuda.device(device):
-        N.check(lib.kdn_sample(a, N.stream_of(logits)), "kdn_sample")
+    N.launch(lib.kdn_sample, a, logits, "kdn_sample")
     return token, prob
 
 

@@ -137,6 +137,24 @@ def test_strided_and_unaligned_rows(D):
 
 
 @pytest.mark.gpu
+def test_broadcast_gate():
+    """One gate row for all rows (stride 0): the same outputs as its copies, and the sum of their gradients."""
+    d = make((2, 6, 40), F, F, "yps", seed=9)
+    x, y, w, p, s = (d[k].cuda() for k in ("x", "y", "weight", "post_weight", "scale"))
+    row = torch.randn(40, device="cuda", requires_grad=True)
+    copies = row.detach().expand(2, 6, 40).contiguous().requires_grad_(True)
+    outs = []
+    for gate in (row.expand(2, 6, 40), copies):
+        z, h = block_norm(x, y, w, post_weight=p, gate=gate, scale=s)
+        outs.append((z, h, torch.autograd.grad(h, row if gate is not copies else copies, d["dh"].cuda())[0]))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    assert nmax(outs[0][2], outs[1][2].sum((0, 1))) < 1e-5
+    z, h = block_norm(x, y, w, gate=row.detach().expand(2, 6, 40))
+    zr, hr = formula(x.double(), y.double(), row.detach().double(), w.double(), None, None)
+    assert nmax(z, zr) < 1e-5 and nmax(h, hr) < 1e-5
+
+
+@pytest.mark.gpu
 def test_empty_rows_zero_rows_and_large_values():
     d = make((0, 48), F, F, "ypgs")
     z, h, grads = ours(d)
@@ -250,7 +268,7 @@ def test_c_entry_refuses_without_launch():
     a.x = a.weight = a.gate = 16
     a.x_stride = a.gate_stride = 32
     assert lib.kdn_block_norm_fwd(a, None) == -1 and b"need a block output" in lib.kdn_last_error()
-    a.gate, a.x_stride = None, 31
+    a.gate, a.x_stride = None, 31  # neither 0 nor a whole row
     assert lib.kdn_block_norm_fwd(a, None) == -1 and b"strides" in lib.kdn_last_error()
     a.x_stride, a.stream_bf16 = 32, 1
     assert lib.kdn_block_norm_fwd(a, None) == -1 and b"fp32 residual stream" in lib.kdn_last_error()
