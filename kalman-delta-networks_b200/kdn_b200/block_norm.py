@@ -35,39 +35,25 @@ def _rows(t, D):
     return t if t.stride(1) == 1 else t.contiguous()
 
 
-def _args(x, y, gate, weight, post_weight, scale, alpha, swish, eps):
-    a = N.KdnBlockNormArgs()
-    a.rows, a.D = x.shape
-    a.alpha, a.eps, a.swish = alpha, eps, swish
-    a.stream_bf16 = x.dtype == torch.bfloat16
-    a.act_bf16 = (x if y is None else y).dtype == torch.bfloat16
-    a.weights_bf16 = weight.dtype == torch.bfloat16
-    a.x, a.x_stride, a.weight = x.data_ptr(), x.stride(0), weight.data_ptr()
-    if y is not None:
-        a.y, a.y_stride = y.data_ptr(), y.stride(0)
-    if gate is not None:
-        a.gate, a.gate_stride = gate.data_ptr(), gate.stride(0)
-    if post_weight is not None:
-        a.post_weight = post_weight.data_ptr()
-    if scale is not None:
-        a.scale = scale.data_ptr()
-    return a
+def _args(x, y, gate, weight, post_weight, scale, z, h, rstd, alpha, swish, eps):
+    """The C arguments (None: absent) in the order of the fields."""
+    return N.KdnBlockNormArgs(
+        x.dtype == torch.bfloat16, (x if y is None else y).dtype == torch.bfloat16, weight.dtype == torch.bfloat16, swish,
+        x.shape[0], x.shape[1], alpha, eps,
+        x.data_ptr(), None if y is None else y.data_ptr(), None if gate is None else gate.data_ptr(),
+        x.stride(0), 0 if y is None else y.stride(0), 0 if gate is None else gate.stride(0),
+        weight.data_ptr(), None if post_weight is None else post_weight.data_ptr(),
+        None if scale is None else scale.data_ptr(), None if z is None else z.data_ptr(),
+        None if h is None else h.data_ptr(), None if rstd is None else rstd.data_ptr())
 
 
 def _forward(x, y, gate, weight, post_weight, scale, alpha, swish, eps, want_rstd):
     """x, y, gate as [rows, D].  Returns (z or None, h, rstd or None), contiguous."""
     lib = N.load_library()
-    a = _args(x, y, gate, weight, post_weight, scale, alpha, swish, eps)
-    z = None
-    if y is not None:
-        z = torch.empty_like(x)
-        a.z = z.data_ptr()
     h = torch.empty_like(x if y is None else y)
-    a.h = h.data_ptr()
-    rstd = None
-    if want_rstd:
-        rstd = x.new_empty((2, x.shape[0]), dtype=torch.float32)
-        a.rstd = rstd.data_ptr()
+    z = None if y is None else torch.empty_like(x)
+    rstd = x.new_empty((2, x.shape[0]), dtype=torch.float32) if want_rstd else None
+    a = _args(x, y, gate, weight, post_weight, scale, z, h, rstd, alpha, swish, eps)
     N.launch(lib.kdn_block_norm_fwd, a, x, "kdn_block_norm_fwd")
     return z, h, rstd
 
@@ -85,27 +71,26 @@ class _BlockNormFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dz, dh):
-        x, y, gate, weight, post_weight, scale, rstd = ctx.saved_tensors
         if dz is None and dh is None:
             return (None,) * 9
-        lib = N.load_library()
-        a = _args(x, y, gate, weight, post_weight, scale, *ctx.meta)
-        a.rstd = rstd.data_ptr()
+        saved = ctx.saved_tensors
+        inputs, needed = saved[:6], ctx.needs_input_grad[:6]
+        a = _args(*inputs, None, None, saved[6], *ctx.meta)
         if dz is not None:
             dz = dz.contiguous()
             a.dz = dz.data_ptr()
         if dh is not None:
             dh = dh.contiguous()
             a.dh = dh.data_ptr()
-        grads = []
-        for t, needed, name in zip((x, y, gate, weight, post_weight, scale), ctx.needs_input_grad,
-                                   ("dx", "dy", "dgate", "dweight", "dpost", "dscale")):
-            needed = needed and not (name == "dweight" and dh is None)  # z does not depend on the weight
-            out = torch.empty_like(t) if needed else None
-            if needed:
-                setattr(a, name, out.data_ptr())
-            grads.append(out)
-        if any(g is not None for g in grads[3:]):
+        else:  # z does not depend on the weight
+            needed = (*needed[:3], False, *needed[4:])
+        grads = [torch.empty_like(t) if n else None for t, n in zip(inputs, needed)]
+        for name, g in zip(("dx", "dy", "dgate", "dweight", "dpost", "dscale"), grads):
+            if g is not None:
+                setattr(a, name, g.data_ptr())
+        lib = N.load_library()
+        x = inputs[0]
+        if any(needed[3:]):
             ws = x.new_empty(lib.kdn_block_norm_workspace_bytes(a.rows, a.D), dtype=torch.uint8)
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
         N.launch(lib.kdn_block_norm_bwd, a, x, "kdn_block_norm_bwd")

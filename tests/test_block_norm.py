@@ -137,6 +137,19 @@ def test_strided_and_unaligned_rows(D):
 
 
 @pytest.mark.gpu
+def test_saved_tensors_may_move():
+    """Saved-tensor hooks that bring the tensors back elsewhere (activation offloading)."""
+    d = make((5, 96), F, F, "ypgs", seed=12)
+    _, _, want = ours(d)
+    with torch.autograd.graph.save_on_cpu():
+        leaves = {k: d[k].cuda().requires_grad_(True) for k in NAMES}
+        z, h = block_norm(leaves["x"], leaves["y"], leaves["weight"], post_weight=leaves["post_weight"],
+                          gate=leaves["gate"], scale=leaves["scale"])
+    got = torch.autograd.grad((z, h), [leaves[k] for k in NAMES], (d["dz"].cuda(), d["dh"].cuda()))
+    assert all(torch.equal(g, want[k]) for g, k in zip(got, NAMES))
+
+
+@pytest.mark.gpu
 def test_broadcast_gate():
     """One gate row for all rows (stride 0): the same outputs as its copies, and the sum of their gradients."""
     d = make((2, 6, 40), F, F, "yps", seed=9)
