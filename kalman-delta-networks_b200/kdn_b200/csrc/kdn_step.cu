@@ -16,10 +16,11 @@
 // rounds to bf16 between its kernels, stay in registers here).
 //
 // Bound by the state's bytes: 8 D^2 per sequence and head, read once and
-// written once.  One CTA holds one head's state in registers (D = 128: 8
-// float4 per thread): the state's loads are issued first and the token's
-// small vectors (3D conv channels, D gates: one thread each) are prepared
-// while they are in flight.
+// written once.  One CTA takes one head's state.  Its copy into shared memory
+// is requested first (cp.async; every thread reads only what it copied), and
+// the token's small vectors (3 D conv channels, D gates: one thread each) are
+// prepared meanwhile.  Three CTAs share an SM (D = 128: 75 KB and 512 threads
+// each), so that one loads while the others compute and store.
 #include "kdn_common.cuh"
 
 namespace kdn {
@@ -40,13 +41,23 @@ __device__ __forceinline__ float ld1(const void* p, size_t i) {
 // D channels per head, 4 D threads: groups of D threads prepare q, k, v and
 // the gates; for the state, D / 4 threads cover a row (float4 each) and 16
 // row groups hold D / 16 consecutive rows each.
+template <int D>
+struct StepShared {
+  float4 state[D * D / 4];        // [row in its group][thread]
+  float part[2][D / 16][D];       // sums of S^T k, S^T q; their totals end in row 0
+  float q[D], k[D], alpha[D], kappa[D];
+  float red[3][D / 32], out[D / 32], scalar[4];
+};
+
 template <int D, bool DIAG, class T>
-__global__ void __launch_bounds__(4 * D, 1024 / (4 * D)) step_kernel(const __grid_constant__ StepParams prm) {
+__global__ void __launch_bounds__(4 * D, D == 128 ? 3 : 6) step_kernel(const __grid_constant__ StepParams prm) {
   const KdnStepArgs& a = prm.a;
-  constexpr int ROWS = D / 16, WG = D / 32, PARTS = D / 8;  // rows per thread, warps per group, warps in all
+  constexpr int ROWS = D / 16, WG = D / 32, HALF = D / 16;  // rows per thread, warps per group, half of the warps
+  extern __shared__ __align__(16) unsigned char raw[];
+  StepShared<D>& sh = *reinterpret_cast<StepShared<D>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t b = blockIdx.x / a.H;
-  const int h = (int)(blockIdx.x - b * a.H);
+  const int64_t b = blockIdx.x / (unsigned)a.H;
+  const int h = (int)(blockIdx.x % (unsigned)a.H);
   const int group = tid / D, d = tid - group * D;
   const size_t C = (size_t)a.H * D;  // channels of one section of qkv
   const size_t ch = (size_t)h * D + d;
@@ -56,31 +67,43 @@ __global__ void __launch_bounds__(4 * D, 1024 / (4 * D)) step_kernel(const __gri
                                      : (int64_t) static_cast<const int32_t*>(a.slots)[b];
   T* y = static_cast<T*>(a.y) + (size_t)b * C + ch;
   if (slot < 0 || slot >= a.num_slots) {  // an idle row: no state, a zero output
-    if (group == 0) *y = from_f<T>(0.f);
+    if (group == 2) *y = from_f<T>(0.f);
     return;
   }
 
   // the state, requested before anything else
   const int c4 = tid % (D / 4), rg = tid / (D / 4);
-  float4* S = reinterpret_cast<float4*>(a.memory + ((size_t)slot * a.H + h) * (D * D)) + c4;
-  float4 st[ROWS];
+  float4* S = reinterpret_cast<float4*>(a.memory + ((size_t)slot * a.H + h) * (D * D)) + rg * ROWS * (D / 4) + c4;
+  float4* held = sh.state + tid;
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) st[i] = S[(size_t)(rg * ROWS + i) * (D / 4)];
-
-  __shared__ __align__(16) float part[2][PARTS][D];  // read and written as float4, like sdelta
-  __shared__ __align__(16) float sdelta[D];
-  __shared__ float sq[D], sk[D], sv[D], sal[D], skap[D], sact[D], sw[D];
-  __shared__ float red[3][WG], sscal[4], sred[WG];
+  for (int i = 0; i < ROWS; ++i) cp_async16(held + i * 4 * D, S + i * (D / 4));
+  cp_async_commit();
 
   // ---- the token's vectors ----
-  float mine = 0.f, prior = 0.f, alpha = 0.f, r = 0.f;
+  float mine = 0.f, prior = 0.f, alpha = 0.f, r = 0.f, act = 0.f;
+  float gate = 0.f, weight = 1.f;
+  if (group == 2) {  // the v threads finish the output: its gate and norm weight stay with them
+    gate = ld1<T>(a.gate, (size_t)b * a.gate_stride + ch);
+    if (a.norm_weight) weight = a.norm_weight[d];
+  }
+  float decay = 0.f, bias = 0.f, log_rate = 0.f, omega = 0.f, noise = 0.f, old = 0.f;
+  if (group == 3) {  // the gates have a group of their own, and with them the diagonal covariance
+    decay = ld1<T>(a.decay_raw, (size_t)b * a.decay_stride + ch);
+    bias = a.dt_bias[ch];
+    log_rate = a.A_log[h];
+    if (DIAG) {
+      omega = ld1<T>(a.omega_raw, (size_t)b * a.omega_stride + ch);
+      noise = ld1<T>(a.r_raw, (size_t)b * a.r_stride + h);
+      old = a.covariance[(size_t)slot * C + ch];
+    }
+  }
   if (group < 3) {
     const size_t gc = (size_t)group * C + ch;
     T* win = static_cast<T*>(a.window) + (size_t)slot * 9 * C + gc;
     const T x3 = static_cast<const T*>(a.qkv)[(size_t)b * a.qkv_stride + gc];
-    const T x1 = win[3 * C], x2 = win[6 * C];
+    const T x0 = win[0], x1 = win[3 * C], x2 = win[6 * C];
     const float4 w = reinterpret_cast<const float4*>(a.conv_weight)[gc];
-    float c = w.x * to_f(win[0]);
+    float c = w.x * to_f(x0);
     c = fmaf(w.y, to_f(x1), c);
     c = fmaf(w.z, to_f(x2), c);
     c = fmaf(w.w, to_f(x3), c);
@@ -89,144 +112,152 @@ __global__ void __launch_bounds__(4 * D, 1024 / (4 * D)) step_kernel(const __gri
     win[6 * C] = x3;
     mine = c * sigmoid_f(c);
   }
-  // the decay: a group of its own (iso); the k threads (diag), which need it
-  // beside k for sum z k^2
-  if (group == (DIAG ? 1 : 3)) {
-    const float f = ld1<T>(a.decay_raw, (size_t)b * a.decay_stride + ch) + a.dt_bias[ch];
-    const float la = -expf(a.A_log[h]) * softplus_f(f);
-    alpha = expf(la);
-  }
+  if (group == 3) alpha = expf(-expf(log_rate) * softplus_f(decay + bias));
+  if (group == 3) sh.alpha[d] = DIAG ? fmaxf(alpha, 1e-6f) : alpha;
   if (DIAG) {
-    if (group == 1) {
-      float* pc = a.covariance + (size_t)slot * C + ch;
-      const float omega = a.omega_min + softplus_f(ld1<T>(a.omega_raw, (size_t)b * a.omega_stride + ch));
-      r = a.r_min + softplus_f(ld1<T>(a.r_raw, (size_t)b * a.r_stride + h));
-      prior = fmaf(alpha * alpha, *pc, omega);
-      sal[d] = fmaxf(alpha, 1e-6f);
-    }
     if (group == 3) {
-      const float g = ld1<T>(a.gate, (size_t)b * a.gate_stride + ch), s = sigmoid_f(g);
-      sact[d] = (a.swish ? g * s : s) * (a.norm_weight ? a.norm_weight[d] : 1.f);
+      r = a.r_min + softplus_f(noise);
+      prior = fmaf(alpha * alpha, old, a.omega_min + softplus_f(omega));
     }
   } else {
-    if (group == 3) sal[d] = alpha;
-    if (group == 2) {
-      const float g = ld1<T>(a.gate, (size_t)b * a.gate_stride + ch), s = sigmoid_f(g);
-      sact[d] = (a.swish ? g * s : s) * (a.norm_weight ? a.norm_weight[d] : 1.f);
-    }
     if (tid == 3 * D) {
-      sscal[0] = a.omega_min + softplus_f(ld1<T>(a.omega_raw, (size_t)b * a.omega_stride + h) + a.omega_bias[h]);
-      sscal[1] = a.r_min + softplus_f(ld1<T>(a.r_raw, (size_t)b * a.r_stride + h) + a.r_bias[h]);
-      sscal[2] = a.covariance[(size_t)slot * a.H + h];
+      sh.scalar[0] = a.omega_min + softplus_f(ld1<T>(a.omega_raw, (size_t)b * a.omega_stride + h) + a.omega_bias[h]);
+      sh.scalar[1] = a.r_min + softplus_f(ld1<T>(a.r_raw, (size_t)b * a.r_stride + h) + a.r_bias[h]);
+      sh.scalar[2] = a.covariance[(size_t)slot * a.H + h];
     }
   }
-  if (group == 0) sq[d] = mine;
-  if (group == 1) sk[d] = mine;
-  if (group == 2) sv[d] = mine;
+  if (group == 0) sh.q[d] = mine;
+  if (group == 1) sh.k[d] = mine;
+  if (group == 2) {
+    const float s = sigmoid_f(gate);
+    act = (a.swish ? gate * s : s) * weight;
+  }
   {
-    // row sums: q^2, k^2 and alpha^2 (iso) or z k^2 (diag, by the k threads)
-    float s = group == 3 ? alpha * alpha : mine * mine;
-    s = warp_sum(s);
-    if (lane == 0 && (group < 2 || (!DIAG && group == 3))) red[group == 3 ? 2 : group][warp % WG] = s;
-    if (DIAG && group == 1) {
-      const float zk = warp_sum(prior * mine * mine);
-      if (lane == 0) red[2][warp % WG] = zk;
-    }
+    // row sums: q^2, k^2 and (iso) alpha^2
+    const float s = warp_sum(group == 3 ? alpha * alpha : mine * mine);
+    if (lane == 0 && (group < 2 || (!DIAG && group == 3))) sh.red[group == 3 ? 2 : group][warp % WG] = s;
   }
   __syncthreads();
 
   float ssq = 0.f, ssk = 0.f, third = 0.f;
 #pragma unroll
   for (int i = 0; i < WG; ++i) {
-    ssq += red[0][i];
-    ssk += red[1][i];
-    third += red[2][i];
+    ssq += sh.red[0][i];
+    ssk += sh.red[1][i];
+    if (!DIAG) third += sh.red[2][i];
   }
-  float rq, rk;
+  float rq, rk, kn = 0.f;
   if (DIAG) {  // the diagonal boundary's norm: x / max(|x|, 1e-12)
     rq = 1.f / fmaxf(sqrtf(ssq), 1e-12f);
     rk = 1.f / fmaxf(sqrtf(ssk), 1e-12f);
-    if (group == 1) {
-      const float kn = mine * rk;
-      skap[d] = prior * kn / (r + third * rk * rk);
-      a.covariance[(size_t)slot * C + ch] = prior / (1.f + (float)D * kn * kn / r * prior);
+    if (group == 3) {  // sum z k^2: published by the next barrier, the gain by the one after it
+      kn = sh.k[d] * rk;
+      const float zk = warp_sum(prior * kn * kn);
+      if (lane == 0) sh.red[2][warp % WG] = zk;
     }
   } else {  // x / sqrt(|x|^2 + 1e-6)
     rq = rsqrtf(ssq + 1e-6f);
     rk = rsqrtf(ssk + 1e-6f);
-    const float om = sscal[0], rr = sscal[1];
-    const float z = fmaf(third * (1.f / (float)D), sscal[2], om);
-    if (group == 1) skap[d] = z / (rr + z) * (mine * rk);
+    const float om = sh.scalar[0], rr = sh.scalar[1];
+    const float z = fmaf(third * (1.f / (float)D), sh.scalar[2], om);
+    if (group == 1) sh.kappa[d] = z / (rr + z) * (mine * rk);
     if (tid == 0) a.covariance[(size_t)slot * a.H + h] = rr * z / fmaf(a.posterior_scale, z, rr);
   }
 
   // ---- one pass over the state: S^ = alpha S, u = S^T k, w = S^T q ----
+  cp_async_wait_all();
   float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int row = rg * ROWS + i;
-    const float al = sal[row], kk = sk[row], qq = sq[row];
-    st[i].x *= al; st[i].y *= al; st[i].z *= al; st[i].w *= al;
-    u.x = fmaf(kk, st[i].x, u.x); u.y = fmaf(kk, st[i].y, u.y);
-    u.z = fmaf(kk, st[i].z, u.z); u.w = fmaf(kk, st[i].w, u.w);
-    w.x = fmaf(qq, st[i].x, w.x); w.y = fmaf(qq, st[i].y, w.y);
-    w.z = fmaf(qq, st[i].z, w.z); w.w = fmaf(qq, st[i].w, w.w);
+    const float4 st = held[i * 4 * D];
+    const float al = sh.alpha[row], kk = sh.k[row] * al, qq = sh.q[row] * al;
+    u.x = fmaf(kk, st.x, u.x); u.y = fmaf(kk, st.y, u.y);
+    u.z = fmaf(kk, st.z, u.z); u.w = fmaf(kk, st.w, u.w);
+    w.x = fmaf(qq, st.x, w.x); w.y = fmaf(qq, st.y, w.y);
+    w.z = fmaf(qq, st.z, w.z); w.w = fmaf(qq, st.w, w.w);
   }
-  if (D == 64) {  // a warp holds two row groups
+  // D / 8 warps: the upper half leaves its sums, the lower half adds its own
+  // (D = 64: a warp holds two row groups, joined first)
+  if (D == 64) {
     u.x += __shfl_xor_sync(0xffffffffu, u.x, 16); u.y += __shfl_xor_sync(0xffffffffu, u.y, 16);
     u.z += __shfl_xor_sync(0xffffffffu, u.z, 16); u.w += __shfl_xor_sync(0xffffffffu, u.w, 16);
     w.x += __shfl_xor_sync(0xffffffffu, w.x, 16); w.y += __shfl_xor_sync(0xffffffffu, w.y, 16);
     w.z += __shfl_xor_sync(0xffffffffu, w.z, 16); w.w += __shfl_xor_sync(0xffffffffu, w.w, 16);
   }
-  if (lane < D / 4) {
-    reinterpret_cast<float4*>(part[0][warp])[c4] = u;
-    reinterpret_cast<float4*>(part[1][warp])[c4] = w;
+  float4* pu = reinterpret_cast<float4*>(sh.part[0][warp % HALF]) + c4;
+  float4* pw = reinterpret_cast<float4*>(sh.part[1][warp % HALF]) + c4;
+  if (warp >= HALF && lane < D / 4) {
+    *pu = u;
+    *pw = w;
   }
   __syncthreads();
-  if (group < 2) {  // D threads finish u and delta, D threads w
-    float s = 0.f;
+  if (DIAG && group == 3) {
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) s += part[group][i][d];
-    if (group == 1)
-      sw[d] = s * rq;
-    else
-      sdelta[d] = sv[d] - s * rk;
+    for (int i = 0; i < WG; ++i) third += sh.red[2][i];
+    sh.kappa[d] = prior * kn / (r + third);
+    a.covariance[(size_t)slot * C + ch] = prior / (1.f + (float)D * kn * kn / r * prior);
   }
-  // q . kappa, by one warp that has no column to sum
-  if (warp == 2 * WG) {
+  if (warp < HALF && lane < D / 4) {
+    const float4 x = *pu, z = *pw;
+    *pu = make_float4(u.x + x.x, u.y + x.y, u.z + x.z, u.w + x.w);
+    *pw = make_float4(w.x + z.x, w.y + z.y, w.z + z.z, w.w + z.w);
+  }
+  __syncthreads();
+  if (group >= 2) {  // the v threads finish u and delta, the gate threads w; a column's threads own it
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < WG; ++i) s = fmaf(sq[lane + 32 * i], skap[lane + 32 * i], s);
+    for (int i = 0; i < HALF; ++i) s += sh.part[group - 2][i][d];
+    if (group == 2) mine -= s * rk;  // delta
+    sh.part[group - 2][0][d] = group == 2 ? mine : s * rq;
+  }
+  if (warp == 0) {  // q . kappa
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < WG; ++i) s = fmaf(sh.q[lane + 32 * i], sh.kappa[lane + 32 * i], s);
     s = warp_sum(s);
-    if (lane == 0) sscal[3] = s * rq;
+    if (lane == 0) sh.scalar[3] = s * rq;
   }
   __syncthreads();
-  const float4 dl = reinterpret_cast<const float4*>(sdelta)[c4];
+  const float4 dl = reinterpret_cast<const float4*>(sh.part[0][0])[c4];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const float ka = skap[rg * ROWS + i];
-    st[i].x = fmaf(ka, dl.x, st[i].x); st[i].y = fmaf(ka, dl.y, st[i].y);
-    st[i].z = fmaf(ka, dl.z, st[i].z); st[i].w = fmaf(ka, dl.w, st[i].w);
-    S[(size_t)(rg * ROWS + i) * (D / 4)] = st[i];
+    const int row = rg * ROWS + i;
+    const float al = sh.alpha[row], ka = sh.kappa[row];
+    float4 st = held[i * 4 * D];
+    st.x = fmaf(ka, dl.x, al * st.x); st.y = fmaf(ka, dl.y, al * st.y);
+    st.z = fmaf(ka, dl.z, al * st.z); st.w = fmaf(ka, dl.w, al * st.w);
+    S[i * (D / 4)] = st;
   }
-  if (group == 0) {
-    const float o = a.scale * fmaf(sscal[3], sdelta[d], sw[d]);
+  if (group == 2) {
+    const float o = a.scale * fmaf(sh.scalar[3], mine, sh.part[1][0][d]);
     const float s = warp_sum(o * o);
-    if (lane == 0) sred[warp] = s;
+    if (lane == 0) sh.out[warp % WG] = s;
     bar_sync(1, D);
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < WG; ++i) ss += sred[i];
-    *y = from_f<T>(o * rsqrtf(ss * (1.f / (float)D) + a.eps) * sact[d]);
+    for (int i = 0; i < WG; ++i) ss += sh.out[i];
+    *y = from_f<T>(o * rsqrtf(ss * (1.f / (float)D) + a.eps) * act);
   }
 }
 
+template <int D, bool DIAG, class T>
+int launch_step(const StepParams& p, unsigned grid, cudaStream_t st) {
+  constexpr size_t smem = sizeof(StepShared<D>);
+  if (smem > 48 * 1024) {
+    const cudaError_t err = cudaFuncSetAttribute(step_kernel<D, DIAG, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (err != cudaSuccess) {
+      cudaGetLastError();
+      return set_error(KDN_ERR_CUDA, "step_kernel: %s", cudaGetErrorString(err));
+    }
+  }
+  step_kernel<D, DIAG, T><<<grid, 4 * D, smem, st>>>(p);
+  return check_launch("step_kernel");
+}
+
 template <int D, class T>
-void launch_step(const StepParams& p, unsigned grid, cudaStream_t st) {
-  if (p.a.variant == KDN_DIAG)
-    step_kernel<D, true, T><<<grid, 4 * D, 0, st>>>(p);
-  else
-    step_kernel<D, false, T><<<grid, 4 * D, 0, st>>>(p);
+int launch_step(const StepParams& p, unsigned grid, cudaStream_t st) {
+  return p.a.variant == KDN_DIAG ? launch_step<D, true, T>(p, grid, st) : launch_step<D, false, T>(p, grid, st);
 }
 
 }  // namespace
@@ -262,12 +293,6 @@ extern "C" int kdn_step(const KdnStepArgs* args, kdn_stream_t stream) {
   StepParams p{a};
   const unsigned grid = (unsigned)(a.B * a.H);
   cudaStream_t st = (cudaStream_t)stream;
-  if (a.D == 128) {
-    if (a.act_bf16) launch_step<128, bf16>(p, grid, st);
-    else launch_step<128, float>(p, grid, st);
-  } else {
-    if (a.act_bf16) launch_step<64, bf16>(p, grid, st);
-    else launch_step<64, float>(p, grid, st);
-  }
-  return check_launch("step_kernel");
+  if (a.D == 128) return a.act_bf16 ? launch_step<128, bf16>(p, grid, st) : launch_step<128, float>(p, grid, st);
+  return a.act_bf16 ? launch_step<64, bf16>(p, grid, st) : launch_step<64, float>(p, grid, st);
 }
