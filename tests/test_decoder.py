@@ -1,0 +1,79 @@
+"""The example model (``kdn_b200.decoder``): training and generation on the package's operators together.
+
+Tolerance of the logits: the whole-sequence path rounds to bf16 after every
+operator (about ten roundings of 2^-9 per layer on the way to the logits, two
+layers), the token path rounds less: 5e-2 of the largest logit.
+"""
+import pytest
+import torch
+
+from kdn_b200.decoder import KDNDecoder
+
+VOCAB, HEADS = 257, 2
+
+
+def make(variant, seed=0, **kw):
+    torch.manual_seed(seed)
+    return KDNDecoder(VOCAB, 192, 2, HEADS, variant=variant, inner=320, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", ["iso", "diag"])
+@pytest.mark.parametrize("kw", [{}, {"post_norm": True, "scale_init": 0.5, "stream": torch.bfloat16}])
+def test_tokens_one_by_one_agree_with_the_whole_sequence(variant, kw):
+    model = make(variant, **kw)
+    tokens = torch.randint(VOCAB, (3, 80), device="cuda")
+    with torch.no_grad():
+        whole = model(tokens).float()
+    pools, steps = model.make_pools(5), [m.make_step() for m in model.mixers]
+    slots = torch.tensor([4, 0, 2], dtype=torch.int32, device="cuda")
+    at = 66  # the prompt ends inside a chunk
+    logits = [model.start(tokens[:, :at], pools, slots.long())]
+    logits += [model.decode(tokens[:, t], pools, steps, slots) for t in range(at, 80)]
+    got = torch.stack(logits, 1).float()
+    want = whole[:, at - 1:]
+    assert (got - want).abs().max() < 5e-2 * want.abs().max()
+    for pool in pools:  # slots that are not in the call stay empty
+        assert (pool.memory[[1, 3]] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", ["iso", "diag"])
+def test_generation_repeats_and_the_graph_changes_nothing(variant):
+    model = make(variant, seed=1)
+    prompts = torch.randint(VOCAB, (4, 5), device="cuda")
+    outs = []
+    for graph in (True, True, False):
+        gen = torch.Generator(device="cuda").manual_seed(3)
+        outs.append(model.generate(prompts, 12, generator=gen, graph=graph, temperature=0.9, top_k=40, top_p=0.9,
+                                   min_p=0.01))
+    for tokens, probs in outs:
+        assert tokens.shape == probs.shape == (4, 12) and tokens.min() >= 0 and tokens.max() < VOCAB
+        assert torch.equal(tokens, outs[0][0]) and torch.equal(probs, outs[0][1])
+    greedy, _ = model.generate(prompts, 3, temperature=0.0)
+    with torch.no_grad():
+        assert torch.equal(greedy[:, 0], model(prompts)[:, -1].float().argmax(-1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", ["iso", "diag"])
+def test_trains(variant):
+    """Ten optimizer steps on one batch: every parameter gets a finite gradient and the loss falls by a third."""
+    model = make(variant, seed=2, post_norm=True, scale_init=1.0)
+    tokens = torch.randint(VOCAB, (2, 65), device="cuda")
+    opt = torch.optim.AdamW(model.parameters(), lr=3e-3)
+    losses = []
+    for _ in range(10):
+        logits = model(tokens[:, :-1])
+        loss = torch.nn.functional.cross_entropy(logits.float().flatten(0, 1), tokens[:, 1:].flatten())
+        opt.zero_grad()
+        loss.backward()
+        assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in model.parameters())
+        opt.step()
+        losses.append(loss.item())
+    assert losses[-1] < losses[0] * 2 / 3, losses
+
+
+def test_refuses_unknown_variants():
+    with pytest.raises(ValueError, match="variant"):
+        KDNDecoder(16, 128, 1, 1, variant="other", device="cpu")
