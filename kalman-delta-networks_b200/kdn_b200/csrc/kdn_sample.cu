@@ -139,8 +139,18 @@ struct Chunk {
   }
 };
 
+// Keys of the largest logit and of two lower bounds: every thread (every warp)
+// holds a token at or above the smallest of the threads' (warps') maxima.
+struct Tops {
+  uint32_t most, least_thread, least_warp;
+};
+__device__ __forceinline__ Tops warp_tops(const Tops& t) {
+  return Tops{__reduce_max_sync(~0u, t.most), __reduce_min_sync(~0u, t.least_thread), __reduce_min_sync(~0u, t.least_warp)};
+}
+
 struct Shared {
   Part warps[kSmWarps], ctas[2][kSmCluster];
+  Tops warp_tops[kSmWarps], cta_tops[kSmCluster];
   uint32_t hist[kBins];
   int least[kSmWarps], most[kSmWarps];  // of a scan: the counts' bounds
   float scan[kSmWarps];
@@ -212,16 +222,47 @@ __global__ void __launch_bounds__(kSmThreads, 3) sample_kernel(const __grid_cons
 #pragma unroll
     for (int k = 0; k < PER; ++k) m = fmaxf(m, v[k]);  // passes over NaN
   });
-  // as a race whose scores are the keys (0: no token), read back as their bits
-  float top = logit_of(__float_as_uint(reduce(Part{Best{__uint_as_float(key_of(m)), 0.f, tid}, 0.f, 0}).best.score));
+  Tops tops{key_of(m), key_of(m), ~0u};
+  tops = warp_tops(tops);
+  tops.least_warp = tops.most;
+  if (lane == 0) sh.warp_tops[warp] = tops;
+  __syncthreads();
+  const Tops none{0u, ~0u, ~0u};
+  if (ctas == 1) {
+    tops = warp_tops(lane < kSmWarps ? sh.warp_tops[lane] : none);
+  } else {
+    if (warp == 0) {
+      tops = warp_tops(lane < kSmWarps ? sh.warp_tops[lane] : none);
+      if (lane < ctas) *cluster.map_shared_rank(&sh.cta_tops[rank], lane) = tops;
+    }
+    cluster.sync();
+    tops = warp_tops(lane < ctas ? sh.cta_tops[lane] : none);
+  }
+  float top = logit_of(tops.most);
+  // with that many threads or warps, a token below their bound is not among the first top_k
+  float floor_l = by_rank && top_k <= kSmWarps * ctas     ? logit_of(tops.least_warp)
+                  : by_rank && top_k <= kSmThreads * ctas ? logit_of(tops.least_thread)
+                                                          : -INFINITY;
   c.infinite = top == INFINITY;
-  if (c.infinite) top = kLargest;
+  if (c.infinite) top = kLargest, floor_l = fminf(floor_l, kLargest);
 
   // ---- 2: Z, and the histogram or the only race ----
   // e = 2^-t, t = (top - l) log2(e) / T in two terms; both are positive, so that -inf gives t = inf, e = 0
   const float scale = __fdiv_rd(1.4426950408889634f, temp);
   const float rest = fmaxf(fmaf(-scale, temp, 1.4426950408889634f) / temp, 1e-30f);
   auto weight = [&](float l) { return fmaxf(ex2a(-fmaf(top - l, scale, (top - l) * rest)), 0.f); };  // NaN: 0
+  // the random numbers of a group: one 32-byte sector, in one round trip
+  const bool noise16 = (reinterpret_cast<uintptr_t>(E) & 15) == 0;
+  auto draw = [&](float (&noise)[PER], int i) {
+    if (PER == 8 && noise16 && i + 8 <= c.end) {
+      const float4 p = __ldg(reinterpret_cast<const float4*>(E + i)), q = __ldg(reinterpret_cast<const float4*>(E + i + 4));
+      noise[0] = p.x; noise[1 % PER] = p.y; noise[2 % PER] = p.z; noise[3 % PER] = p.w;
+      noise[4 % PER] = q.x; noise[5 % PER] = q.y; noise[6 % PER] = q.z; noise[7 % PER] = q.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < PER; ++k) noise[k] = i + k < c.end ? __ldg(E + i + k) : 1.f;
+    }
+  };
   Best best = nobody;
   auto enter = [&](float e, float noise, float l, int i) {  // a thread's indexes grow: ties stay with the first
     const float score = __fdividef(e, noise);
@@ -229,7 +270,6 @@ __global__ void __launch_bounds__(kSmThreads, 3) sample_kernel(const __grid_cons
   };
   float Z = 0.f;
   if (!greedy && top > -INFINITY) {
-    const bool noise16 = VEC && ((reinterpret_cast<uintptr_t>(E) & 15) == 0);
     c.each([&](const float (&v)[PER], int i) {
       float e[PER];
 #pragma unroll
@@ -241,18 +281,11 @@ __global__ void __launch_bounds__(kSmThreads, 3) sample_kernel(const __grid_cons
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
           const uint32_t u = __float_as_uint(e[k]) - 1, bin = (kOne - 1 - u) >> kBinShift;
-          if (bin < kBins) atomicAdd(&sh.hist[bin], ((u & 0x7fffffu) | 0x800000u) >> (8 + down));
+          if (bin < kBins && v[k] >= floor_l) atomicAdd(&sh.hist[bin], ((u & 0x7fffffu) | 0x800000u) >> (8 + down));
         }
       } else {
         float noise[PER];
-        if (PER == 8 && noise16 && i + 8 <= c.end) {
-          const float4 p = __ldg(reinterpret_cast<const float4*>(E + i)), q = __ldg(reinterpret_cast<const float4*>(E + i + 4));
-          noise[0] = p.x; noise[1 % PER] = p.y; noise[2 % PER] = p.z; noise[3 % PER] = p.w;
-          noise[4 % PER] = q.x; noise[5 % PER] = q.y; noise[6 % PER] = q.z; noise[7 % PER] = q.w;
-        } else {
-#pragma unroll
-          for (int k = 0; k < PER; ++k) noise[k] = i + k < c.end ? E[i + k] : 1.f;
-        }
+        draw(noise, i);
 #pragma unroll
         for (int k = 0; k < PER; ++k)
           if (e[k] >= min_p) enter(e[k], noise[k], v[k], i + k);
@@ -286,8 +319,8 @@ __global__ void __launch_bounds__(kSmThreads, 3) sample_kernel(const __grid_cons
     }
     int pl_ = least[0] + least[1], pm_ = most[0] + most[1];  // inclusive scans over the threads
     float ps_ = mass[0] + mass[1];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1) {  // (rolled up: the code is run once, and its instructions come from memory)
       const int x = __shfl_up_sync(~0u, pl_, o), y = __shfl_up_sync(~0u, pm_, o);
       const float f = __shfl_up_sync(~0u, ps_, o);
       if (lane >= o) pl_ += x, pm_ += y, ps_ += f;
@@ -313,8 +346,11 @@ __global__ void __launch_bounds__(kSmThreads, 3) sample_kernel(const __grid_cons
     cut = __reduce_min_sync(~0u, sh.cut[lane % kSmWarps]);
     safe = __reduce_max_sync(~0u, sh.safe[lane % kSmWarps]);
     // tokens of bins before b have e above these
-    const float e_cut = cut == kBins ? 0.f : __uint_as_float(kOne - ((uint32_t)cut << kBinShift));
-    const float e_safe = fmaxf(__uint_as_float(kOne - ((uint32_t)safe << kBinShift)), e_cut);
+    // tokens below floor_l are not in the histogram: they are dropped, and nothing above it has one ahead
+    const float e_floor = floor_l > -INFINITY ? weight(floor_l) : 0.f;
+    const float e_cut = fmaxf(cut == kBins ? 0.f : __uint_as_float(kOne - ((uint32_t)cut << kBinShift)),
+                              e_floor > 0.f ? __uint_as_float(__float_as_uint(e_floor) - 1) : 0.f);
+    const float e_safe = fmaxf(__uint_as_float(kOne - ((uint32_t)safe << kBinShift)), fmaxf(e_cut, e_floor));
 
     // What a turn looks at lies ahead of (pl, pi) in the order.
     float pl = -INFINITY;
@@ -331,13 +367,15 @@ __global__ void __launch_bounds__(kSmThreads, 3) sample_kernel(const __grid_cons
 #pragma unroll
         for (int k = 1; k < PER; ++k) most_l = fmaxf(most_l, v[k]);
         if (most_l < pl || !(weight(most_l) > e_cut)) return;
+        float noise[PER];
+        draw(noise, i);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          const float l = v[k], e = weight(l);
-          if (ahead(l, i + k, pl, pi) && e > e_cut) {
+          const float e = weight(v[k]);
+          if (e > e_cut && ahead(v[k], i + k, pl, pi)) {
             weights += e;
             ++count;
-            if (e >= min_p) enter(e, E[i + k], l, i + k);
+            if (e >= min_p) enter(e, noise[k], v[k], i + k);
           }
         }
       });
