@@ -21,7 +21,7 @@
 // added in a fixed order by a second kernel.
 #pragma once
 
-#include "kdn_common.cuh"
+#include "kdn_launch.cuh"
 
 namespace kdn {
 namespace {
@@ -434,22 +434,16 @@ struct BnRing {
   }
 };
 
-template <class K>
-int bn_start(K* kernel, BnParams p, const BnGeom& g, int weight_planes, size_t fixed, const char* what, cudaStream_t st) {
+template <auto Kernel>
+int bn_start(BnParams p, const BnGeom& g, int weight_planes, size_t fixed, const char* what, cudaStream_t st) {
   const size_t threads = (size_t)g.tpr * g.rpb, places = (size_t)(p.a.D + kBnVec - 1) / kBnVec + 1;
   const size_t plane = sizeof(uint4) * places * g.rpb, weights = sizeof(float4) * weight_planes * places;
   p.stages = (int)((kBnSmem - fixed - weights) / (plane * p.planes));
   if (p.stages < 1) return set_error(KDN_ERR_INVALID, "%s: a row does not fit shared memory", what);
   if (p.stages > 4) p.stages = 4;
   const size_t smem = weights + p.stages * p.planes * plane;
-  if (smem > 40 * 1024) {  // with the static part, more than a launch gets unasked
-    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (err != cudaSuccess) {
-      cudaGetLastError();
-      return set_error(KDN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
-    }
-  }
-  kernel<<<g.grid, (unsigned)threads, smem, st>>>(p);
+  if (int rc = allow_smem<Kernel>(kBnSmem - fixed, what)) return rc;
+  Kernel<<<g.grid, (unsigned)threads, smem, st>>>(p);
   return check_launch(what);
 }
 

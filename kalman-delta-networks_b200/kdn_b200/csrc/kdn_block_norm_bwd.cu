@@ -247,9 +247,9 @@ template <class TX, class TY, bool FULL, bool ALIGNED>
 int bwd_sizes(const BnParams& p, const BnGeom& g, cudaStream_t st) {
   const char* what = "block_norm_bwd_kernel";
   constexpr size_t fixed = sizeof(float) * kBnGroups * 2 * (FULL ? 3 : 1) * kBnRed;
-  if (g.slots == 1) return bn_start(block_norm_bwd_kernel<TX, TY, 1, FULL, ALIGNED>, p, g, kWeightPlanes<FULL>, fixed, what, st);
-  if (g.slots == 2) return bn_start(block_norm_bwd_kernel<TX, TY, 2, FULL, ALIGNED>, p, g, kWeightPlanes<FULL>, fixed, what, st);
-  return bn_start(block_norm_bwd_kernel<TX, TY, 3, FULL, ALIGNED>, p, g, kWeightPlanes<FULL>, fixed, what, st);
+  if (g.slots == 1) return bn_start<block_norm_bwd_kernel<TX, TY, 1, FULL, ALIGNED>>(p, g, kWeightPlanes<FULL>, fixed, what, st);
+  if (g.slots == 2) return bn_start<block_norm_bwd_kernel<TX, TY, 2, FULL, ALIGNED>>(p, g, kWeightPlanes<FULL>, fixed, what, st);
+  return bn_start<block_norm_bwd_kernel<TX, TY, 3, FULL, ALIGNED>>(p, g, kWeightPlanes<FULL>, fixed, what, st);
 }
 
 template <class TX, class TY>

@@ -22,7 +22,7 @@
 // top-k and top-p race in step 2.  Sums have a fixed order or are integers.
 #include <cooperative_groups.h>
 
-#include "kdn_common.cuh"
+#include "kdn_launch.cuh"
 
 namespace kdn {
 namespace {
@@ -449,13 +449,7 @@ int sample_launch(const KdnSampleArgs& a, cudaStream_t st) {
   const int64_t group = kSmThreads * Chunk<T, VEC>::kPer, most = kSmHeld / (group * (int64_t)sizeof(T));
   const int64_t need = (chunk + group - 1) / group, groups = need < most ? need : most;
   const size_t smem = (size_t)(groups * group) * sizeof(T);
-  if (smem > 40 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(sample_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (err != cudaSuccess) {
-      cudaGetLastError();
-      return set_error(KDN_ERR_CUDA, "sample_kernel: %s", cudaGetErrorString(err));
-    }
-  }
+  if (int rc = allow_smem<sample_kernel<T, VEC>>(kSmHeld, "sample_kernel")) return rc;
   int down = 0;  // a bin's entry, below 2^16 >> down per token, fits 32 bits
   while ((chunk << 16 >> down) >> 32) ++down;
   cudaLaunchConfig_t cfg{};

@@ -21,7 +21,7 @@
 // the token's small vectors (3 D conv channels, D gates: one thread each) are
 // prepared meanwhile.  Three CTAs share an SM (D = 128: 75 KB and 512 threads
 // each), so that one loads while the others compute and store.
-#include "kdn_common.cuh"
+#include "kdn_launch.cuh"
 
 namespace kdn {
 namespace {
@@ -244,13 +244,7 @@ __global__ void __launch_bounds__(4 * D, D == 128 ? 3 : 6) step_kernel(const __g
 template <int D, bool DIAG, class T>
 int launch_step(const StepParams& p, unsigned grid, cudaStream_t st) {
   constexpr size_t smem = sizeof(StepShared<D>);
-  if (smem > 48 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(step_kernel<D, DIAG, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (err != cudaSuccess) {
-      cudaGetLastError();
-      return set_error(KDN_ERR_CUDA, "step_kernel: %s", cudaGetErrorString(err));
-    }
-  }
+  if (int rc = allow_smem<step_kernel<D, DIAG, T>>(smem, "step_kernel")) return rc;
   step_kernel<D, DIAG, T><<<grid, 4 * D, smem, st>>>(p);
   return check_launch("step_kernel");
 }

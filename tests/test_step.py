@@ -350,6 +350,6 @@ def test_c_entry_refuses_without_launch():
     assert lib.kdn_step(a, None) == -1 and b"16-byte aligned" in lib.kdn_last_error()
     a.memory, a.num_slots = 16, 0
     assert lib.kdn_step(a, None) == -1 and b"pool must hold" in lib.kdn_last_error()
-    a.B, a.num_slots = 2, 2
+    a.B, a.num_slots, a.qkv_stride = 2, 2, 100  # neither 0 (one row for all) nor a whole row
     assert lib.kdn_step(a, None) == -1 and b"strides" in lib.kdn_last_error()
     assert ctypes.sizeof(N.KdnStepArgs) == 16 + 4 * 8 + 5 * 8 + 5 * 8 + 6 * 8 + 5 * 4 + 4 + 5 * 8
