@@ -7,6 +7,7 @@ missing.  There is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -234,6 +235,30 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_HOST_ENTRIES = ("kdn_step", "kdn_block_norm_fwd", "kdn_block_norm_bwd", "kdn_block_norm_workspace_bytes", "kdn_sample",
+                 "kdn_last_error")
+_host = None
+
+
+def host():
+    """The C++ host path of the token step, the block norms and the sampling (``csrc/host/kdn_torch.cpp``): their
+    functions answer None for what they leave to the Python path.  None where it is not built, or with
+    ``KDN_B200_HOST=python``; both paths make the same calls into the C library."""
+    global _host
+    if _host is None:
+        path = os.path.join(_HERE, "lib", "_kdn_torch.so")
+        if os.environ.get("KDN_B200_HOST", "") == "python" or not os.path.exists(path):
+            _host = False
+        else:
+            spec = importlib.util.spec_from_file_location("_kdn_torch", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            lib = load_library()
+            module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _HOST_ENTRIES))
+            _host = module
+    return _host or None
 
 
 def launch(entry, args, t: torch.Tensor, what: str) -> None:

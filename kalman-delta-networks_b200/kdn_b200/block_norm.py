@@ -142,6 +142,12 @@ def block_norm(x, y, weight, *, post_weight=None, gate=None, scale=None, alpha=1
     is x itself and h = norm(x) * weight.  Differentiable in every tensor.
     """
     alpha, eps = float(alpha), float(eps)
+    fast = N.host()
+    if fast is not None and y is not None and weight is not None and activation in _ACTIVATIONS:
+        out = fast.block_norm(x, y, weight, post_weight, gate, scale, alpha, _ACTIVATIONS[activation], eps, MIN_WIDTH,
+                              MAX_WIDTH)
+        if out is not None:
+            return out
     D = _validate(x, y, weight, post_weight, gate, scale, alpha, activation)
     swish = _ACTIVATIONS[activation]
     shape = x.shape

@@ -2,7 +2,9 @@
 
 Each translation unit is compiled in parallel to ``_build/*.o`` and linked
 into one shared library exporting the C ABI declared in ``include/kdn_b200.h``.
-Rebuilds only when a source or header is newer than the library.
+Beside it g++ builds ``lib/_kdn_torch.so`` from ``csrc/host``: the C++ host
+path of the serving operators (``_native.host``).  Rebuilds only when a source
+or header is newer than the libraries.
 
     python -m kdn_b200.build [--force]
 """
@@ -19,6 +21,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libkdn_b200.so")
+HOST_SRC = os.path.join(CSRC, "host", "kdn_torch.cpp")
+HOST_LIB = os.path.join(LIB_DIR, "_kdn_torch.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 INCLUDE = os.path.abspath(os.path.join(HERE, "..", "..", "include"))
 
@@ -41,19 +45,58 @@ def _deps():
     return _sources() + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h")) + [__file__]
 
 
+def _newer(lib: str, deps) -> bool:
+    return os.path.exists(lib) and all(os.path.getmtime(d) <= os.path.getmtime(lib) for d in deps)
+
+
 def up_to_date() -> bool:
-    if not os.path.exists(LIB):
-        return False
-    t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(d) <= t for d in _deps())
+    return _newer(LIB, _deps())
+
+
+def host_up_to_date() -> bool:
+    return _newer(HOST_LIB, [HOST_SRC, __file__] + glob.glob(os.path.join(INCLUDE, "*.h")))
+
+
+def build_host(verbose: bool = False) -> str:
+    """The C++ host path, against the running torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = ["g++", "-O2", "-fPIC", "-shared", "-std=c++17", "-DTORCH_EXTENSION_NAME=_kdn_torch",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for path in include:
+        cmd += ["-isystem", path]
+    cmd += [HOST_SRC, "-o", HOST_LIB + ".tmp"]
+    cmd += [f"-L{path}" for path in cpp_extension.library_paths()]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {os.path.basename(HOST_SRC)}:\n{res.stderr}")
+    os.replace(HOST_LIB + ".tmp", HOST_LIB)
+    return HOST_LIB
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and up_to_date():
-        return LIB
-    nvcc = _nvcc()
+    """Build what is out of date; returns the C library's path."""
     os.makedirs(BUILD_DIR, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
+    with concurrent.futures.ThreadPoolExecutor(max_workers=1) as pool:  # beside the kernels
+        host = None if not force and host_up_to_date() else pool.submit(build_host, verbose)
+        if force or not up_to_date():
+            _build_kernels(verbose)
+        if host is not None:
+            host.result()
+    return LIB
+
+
+def _build_kernels(verbose: bool) -> None:
+    nvcc = _nvcc()
 
     def compile_one(src: str) -> str:
         obj = os.path.join(BUILD_DIR, os.path.basename(src)[:-3] + ".o")
@@ -73,7 +116,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stderr}")
     os.replace(tmp, LIB)
-    return LIB
 
 
 if __name__ == "__main__":

@@ -46,6 +46,11 @@ def sample(logits, noise, *, temperature=1.0, top_k=None, top_p=None, min_p=None
     top_k <= 0 or top_p >= 1: no such filter.  temperature <= 0: the most likely token, prob 1.  NaN logits count as -inf and +inf as the
     largest fp32 value; a row with nothing above -inf gives token -1, prob 0.
     """
+    fast = N.host()
+    if fast is not None:
+        out = fast.sample(logits, noise, temperature, top_k, top_p, min_p, _VOCAB_LIMIT)
+        if out is not None:
+            return out
     if logits.ndim != 2 or not 1 <= logits.shape[1] <= _VOCAB_LIMIT:
         raise ValueError(f"logits must be [rows, V] with V >= 1, got {tuple(logits.shape)}")
     if logits.dtype not in (torch.bfloat16, torch.float32):
