@@ -159,7 +159,7 @@ extern "C" int kdn_block_norm_fwd(const KdnBlockNormArgs* args, kdn_stream_t str
   const KdnBlockNormArgs& a = *args;
   if (a.rows == 0) return KDN_OK;
   if (!a.h || (a.y && !a.z)) return set_error(KDN_ERR_INVALID, "kdn_block_norm_fwd: null output");
-  const BnGeom g = bn_geom(a.rows, a.D, bn_aligned(a) ? kBnBwdWarps : kBnFwdWarps);
+  const BnGeom g = bn_geom(a.rows, a.D, bn_aligned(a) ? kBnBwdWarps : kBnFwdWarps, true);
   const int ex = a.stream_bf16 ? 1 : 2, ey = a.act_bf16 ? 1 : 2;
   const BnParams p{a, nullptr, g.tpr, ex + (a.y ? ey : 0) + (a.gate ? ey : 0), 0};
   cudaStream_t st = (cudaStream_t)stream;

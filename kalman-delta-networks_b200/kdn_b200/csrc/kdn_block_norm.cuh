@@ -31,10 +31,13 @@ constexpr int kBnMaxD = 8192;
 constexpr int kBnMinD = 2;  // the norm of one value is its sign: fp32 cannot resolve its gradient (of the order of eps)
 // A row belongs to the fewest warps whose lanes hold it in three slots each:
 // what a row costs beside its values (reductions, addresses, barriers) is paid
-// per warp.  One CTA per SM with as many rows at a time as its warps make: 12
-// warps, or 16 in the forward of unaligned rows, which shift their pieces and
-// wait at a barrier per row (8192 x 2305 bf16, all parts: 78 us against 90
-// with 12; aligned 16384 x 2304: 71 against 67).
+// per warp.  The backward of unaligned rows (dense false) takes as few slots as
+// the CTA's warps allow instead: every slot's shifts are code of its own, more
+// of it than registers and instruction fetch bear (1000 x 1155 fp32: 31 us
+// against 39; 8192 x 2305 bf16: 203 against 218; the forward loses, 125 us
+// against 79).  One CTA per SM with as many rows at a time as its
+// warps make: 12 warps (168 registers a thread), in the forward of unaligned
+// rows, which wait at a barrier per row, 16.
 constexpr int kBnFwdWarps = 16, kBnBwdWarps = 12, kBnSlots = 3;
 constexpr size_t kBnSmem = 232448;  // a CTA's shared memory; fp32 rows of 8192 values and their weights fit once
 
@@ -45,9 +48,11 @@ struct BnGeom {
   unsigned grid;
 };
 
-inline BnGeom bn_geom(int64_t rows, int64_t D, int cta_warps) {
+inline BnGeom bn_geom(int64_t rows, int64_t D, int cta_warps, bool dense) {
   BnGeom g;
-  const int nv = (int)((D + kBnVec - 1) / kBnVec), warps = (nv + 32 * kBnSlots - 1) / (32 * kBnSlots);
+  const int nv = (int)((D + kBnVec - 1) / kBnVec);
+  g.slots = dense ? kBnSlots : (nv + 32 * cta_warps - 1) / (32 * cta_warps);
+  const int warps = (nv + 32 * g.slots - 1) / (32 * g.slots);
   g.tpr = 32 * warps;
   g.slots = (nv + g.tpr - 1) / g.tpr;
   g.rpb = cta_warps / warps;
@@ -380,7 +385,7 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* red, int& phase,
   for (int i = 0; i < N; ++i) {
     v[i] = 0.f;
 #pragma unroll
-    for (int q = 0; q < 3; ++q) {  // a row has at most 11 warps
+    for (int q = 0; q < kBnRed / 4; ++q) {
       const float4 f = reinterpret_cast<const float4*>(r + i * kBnRed)[q];
       v[i] += (f.x + f.y) + (f.z + f.w);
     }

@@ -268,8 +268,9 @@ extern "C" {
 
 size_t kdn_block_norm_workspace_bytes(int64_t rows, int64_t D) {
   if (rows <= 0 || D < kBnMinD || D > kBnMaxD) return 0;
-  const BnGeom g = bn_geom(rows, D, kBnBwdWarps);
-  return align_up(sizeof(float) * 2 * (size_t)D * g.grid, 256);
+  // the larger of the two geometries' grids
+  const unsigned a = bn_geom(rows, D, kBnBwdWarps, true).grid, b = bn_geom(rows, D, kBnBwdWarps, false).grid;
+  return align_up(sizeof(float) * 2 * (size_t)D * (a > b ? a : b), 256);
 }
 
 int kdn_block_norm_bwd(const KdnBlockNormArgs* args, kdn_stream_t stream) {
@@ -288,7 +289,7 @@ int kdn_block_norm_bwd(const KdnBlockNormArgs* args, kdn_stream_t stream) {
     return set_error(KDN_ERR_INVALID, "kdn_block_norm_bwd: a gradient of an absent input");
   if (weights && (!a.workspace || a.workspace_bytes < kdn_block_norm_workspace_bytes(a.rows, a.D)))
     return set_error(KDN_ERR_WORKSPACE, "kdn_block_norm_bwd: workspace too small");
-  const BnGeom g = bn_geom(a.rows, a.D, kBnBwdWarps);
+  const BnGeom g = bn_geom(a.rows, a.D, kBnBwdWarps, bn_aligned(a));
   const int ex = a.stream_bf16 ? 1 : 2, ey = a.act_bf16 ? 1 : 2;
   const BnParams p{a, weights ? static_cast<float*>(a.workspace) : nullptr, g.tpr,
                    2 * ex + (a.y ? 2 : 1) * ey + (a.gate ? ey : 0), 0};
