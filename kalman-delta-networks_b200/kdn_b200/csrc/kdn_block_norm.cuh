@@ -19,6 +19,10 @@
 // Rows that do not start on 16-byte boundaries are copied as the aligned
 // pieces that cover them and shifted when they are read.  The groups' sums are
 // added in a fixed order by a second kernel.
+//
+// 16384 x 2304 bf16: all parts 68 us forward (5.5 TB/s) and 116 us backward
+// (5.2 TB/s, the second kernel included), the plain sum 55 and 87 us; with an
+// fp32 stream 99 / 153 and 84 / 126 us.
 #pragma once
 
 #include "kdn_launch.cuh"
