@@ -681,15 +681,15 @@ int kdn_block_norm_bwd(const KdnBlockNormArgs* args, kdn_stream_t stream);
  *   prob = e_token / Z
  *
  * so that a kept token is drawn with probability e_i / sum of the kept e.
- * T <= 0: the first of the order, prob 1.  NaN logits count as -inf, +inf
- * as the largest fp32 value; a row with nothing above -inf gives token -1,
- * prob 0.  top_k <= 0: no limit.
+ * T below 1e-37 (0, negative, NaN): the first of the order, prob 1.  NaN
+ * logits count as -inf, +inf as the largest fp32 value; a row with nothing
+ * above -inf gives token -1, prob 0.  top_k <= 0: no limit.
  * temperature, top_p, min_p: fp32 [rows] or NULL with the value for all rows
  * beside it; top_k: int32 [rows] (int64 if top_k_i64) or NULL likewise.
  * logits: bf16 (logits_bf16) or fp32, noise fp32, with row strides (elements; 0:
  * one row for all).
- * token: int64 [rows], prob: fp32 [rows].  V <= 2^29.  Workspace:
- * kdn_sample_workspace_bytes(rows, V).  Zero-initialise the struct.
+ * token: int64 [rows], prob: fp32 [rows].  V <= 2^29.  Zero-initialise the
+ * struct.
  * ------------------------------------------------------------------------ */
 typedef struct KdnSampleArgs {
   int32_t logits_bf16, top_k_i64;
@@ -706,11 +706,8 @@ typedef struct KdnSampleArgs {
   float top_p_all, min_p_all;
   int64_t* token;
   float* prob;
-  void* workspace;
-  size_t workspace_bytes;
 } KdnSampleArgs;
 
-size_t kdn_sample_workspace_bytes(int64_t rows, int64_t V);
 int kdn_sample(const KdnSampleArgs* args, kdn_stream_t stream);
 
 #ifdef __cplusplus

@@ -107,8 +107,7 @@ KdnSampleArgs = _struct(
     (ctypes.c_float, "temperature_all"),
     (ctypes.c_int64, "top_k_all"),
     (ctypes.c_float, "top_p_all min_p_all"),
-    (ctypes.c_void_p, "token prob workspace"),
-    (ctypes.c_size_t, "workspace_bytes"),
+    (ctypes.c_void_p, "token prob"),
 )
 
 _P = ctypes.c_void_p
@@ -184,7 +183,6 @@ _SIGNATURES = {
     "kdn_block_norm_workspace_bytes": ([_I64, _I64], _SZ),
     "kdn_block_norm_fwd": ([ctypes.POINTER(KdnBlockNormArgs), _P], ctypes.c_int),
     "kdn_block_norm_bwd": ([ctypes.POINTER(KdnBlockNormArgs), _P], ctypes.c_int),
-    "kdn_sample_workspace_bytes": ([_I64, _I64], _SZ),
     "kdn_sample": ([ctypes.POINTER(KdnSampleArgs), _P], ctypes.c_int),
 }
 

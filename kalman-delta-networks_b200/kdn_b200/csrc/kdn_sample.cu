@@ -40,6 +40,7 @@ constexpr int kSmHeld = 192 * 1024;  // bytes of shared memory for them; what a 
 constexpr int kSmCluster = 8;
 constexpr int kRaces = 12;
 constexpr float kLargest = 3.402823466e38f;
+constexpr float kColdest = 1e-37f;  // log2(e) / T is finite from here on; what is below (0, negative, NaN) is greedy
 constexpr int kBins = 1024;      // e from 1 down to 2^-64
 constexpr int kBinShift = 23 - 4;  // 16 bins per octave
 constexpr uint32_t kOne = 0x3f800000u;  // the bits of e = 1
@@ -203,6 +204,8 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const __grid_cons
     buf ^= 1;
     return p;
   };
+  // The CTAs write into each other's memory: all of them have to have started.  Waited for before the first write.
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   Tokens c;
   c.row = static_cast<const T*>(a.logits) + row * a.logits_stride;
   c.begin = (int)min((int64_t)rank * chunk, (int64_t)V);
@@ -216,7 +219,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const __grid_cons
                   : a.top_k_i64 ? static_cast<const int64_t*>(a.top_k)[row]
                                 : (int64_t) static_cast<const int32_t*>(a.top_k)[row];
   const int top_k = limit <= 0 || limit > V ? V : (int)limit;
-  const bool greedy = !(temp > 0.f), by_rank = !greedy && (top_k < V || top_p < 1.f);
+  const bool greedy = !(temp >= kColdest), by_rank = !greedy && (top_k < V || top_p < 1.f);
   const float* E = a.noise + row * a.noise_stride;
   for (int i = tid; i < kBins; i += kSmThreads) sh.hist[i] = 0;
   cp_async_wait_all();
@@ -236,6 +239,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const __grid_cons
   if (ctas == 1) {
     tops = warp_tops(lane < kSmWarps ? sh.warp_tops[lane] : none);
   } else {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (warp == 0) {
       tops = warp_tops(lane < kSmWarps ? sh.warp_tops[lane] : none);
       if (lane < ctas) *cluster.map_shared_rank(&sh.cta_tops[rank], lane) = tops;
@@ -482,12 +486,6 @@ int sample_launch(const KdnSampleArgs& a, cudaStream_t st) {
 using namespace kdn;
 
 extern "C" {
-
-size_t kdn_sample_workspace_bytes(int64_t rows, int64_t V) {
-  (void)rows;
-  (void)V;
-  return 0;
-}
 
 int kdn_sample(const KdnSampleArgs* args, kdn_stream_t stream) {
   if (!args) return set_error(KDN_ERR_INVALID, "kdn_sample: null args");

@@ -43,8 +43,8 @@ def sample(logits, noise, *, temperature=1.0, top_k=None, top_p=None, min_p=None
 
     logits [rows, V] bf16 or fp32 and noise [rows, V] fp32 (positive), rows contiguous with any row stride.
     temperature, top_p, min_p: numbers or fp32 tensors [rows]; top_k: int or int32 / int64 tensor [rows]; None,
-    top_k <= 0 or top_p >= 1: no such filter.  temperature <= 0: the most likely token, prob 1.  NaN logits count as -inf and +inf as the
-    largest fp32 value; a row with nothing above -inf gives token -1, prob 0.
+    top_k <= 0 or top_p >= 1: no such filter.  temperature below 1e-37 (0, negative): the most likely token, prob 1.
+    NaN logits count as -inf and +inf as the largest fp32 value; a row with nothing above -inf gives token -1, prob 0.
     """
     fast = N.host()
     if fast is not None:

@@ -148,6 +148,25 @@ def test_extreme_noise():
 
 
 @pytest.mark.gpu
+def test_extreme_parameters():
+    """Temperatures from below the fp32 range of 1 / T to infinity, thresholds outside [0, 1]: always a token of the
+    row, and the most likely one where the definition leaves no other."""
+    V = 3000
+    logits, noise = make(1, V, torch.float32, seed=21)
+    first = logits[0].argmax().item()
+    T = torch.tensor([0.0, -1.0, math.nan, 1e-45, 1e-38, 1e-36, 1e-20, 1e-3])
+    token, prob = sample(logits.expand(8, V).cuda(), noise.expand(8, V).cuda(), temperature=T.cuda())
+    assert (token == first).all() and (prob == 1).all()
+    token, prob = sample(logits.cuda(), noise.cuda(), temperature=math.inf)  # an even draw
+    assert token[0] == (1 / noise[0]).argmax() and abs(prob[0].item() * V - 1) < 1e-5
+    for options in ({"top_p": 0.0}, {"top_p": -1.0}, {"min_p": 1.5}, {"min_p": math.inf}, {"top_k": 1, "top_p": 0.0}):
+        token, _ = sample(logits.cuda(), noise.cuda(), **options)
+        assert token[0] == first, options
+    for options in ({"top_p": 2.0}, {"top_p": math.inf}, {"min_p": -1.0}, {"top_k": -3}, {"top_k": V + 1}):
+        assert torch.equal(sample(logits.cuda(), noise.cuda(), **options)[0], sample(logits.cuda(), noise.cuda())[0])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("options", [{}, {"top_k": 4}, {"top_p": 0.7}])
 def test_winner_always_last_of_the_order(options):
     """Noise that favours the rear of the order at every turn, so that every race is lost to a later token."""
