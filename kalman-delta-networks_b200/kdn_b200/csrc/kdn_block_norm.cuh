@@ -49,19 +49,39 @@ struct BnGeom {
   int slots;  // slots per thread: 1, 2 or 3
   int tpr;    // threads per row
   int rpb;    // rows per CTA at a time
+  int period;  // rows from one to the next of the same shift
   unsigned grid;
 };
 
-inline BnGeom bn_geom(int64_t rows, int64_t D, int cta_warps, bool dense) {
+// How the rows of a call lie in memory.  Aligned: every row starts on a 16-byte
+// boundary and is a whole number of vectors.  Packed: rows of another width, in
+// tensors that are contiguous and aligned as a whole.  A row's vectors are then
+// the aligned words of memory that cover it, its first column `shift` places
+// into the first one, and rows a `period` apart have the same shift: a CTA takes
+// rows of one shift only, so that its weights and its columns' sums are those of
+// aligned rows, moved by it; only the outer vectors of a row differ (what they
+// hold of the neighbours is cleared in shared memory, their values are stored
+// one by one).  Loose: any other strides and alignments.
+enum BnRows { kBnLoose = 0, kBnAligned = 1, kBnPacked = 2 };
+
+// vectors of a row (packed: of the rows with the largest shift)
+__host__ __device__ inline int bn_vectors(int D, bool packed) {
+  return packed && D % kBnVec ? (D + 2 * kBnVec - 2) / kBnVec : (D + kBnVec - 1) / kBnVec;
+}
+
+inline BnGeom bn_geom(int64_t rows, int64_t D, int cta_warps, BnRows kind, bool few_slots) {
   BnGeom g;
-  const int nv = (int)((D + kBnVec - 1) / kBnVec);
-  g.slots = dense ? kBnSlots : (nv + 32 * cta_warps - 1) / (32 * cta_warps);
+  const int nv = bn_vectors((int)D, kind == kBnPacked);
+  g.slots = !few_slots ? kBnSlots : (nv + 32 * cta_warps - 1) / (32 * cta_warps);
   const int warps = (nv + 32 * g.slots - 1) / (32 * g.slots);
   g.tpr = 32 * warps;
   g.slots = (nv + g.tpr - 1) / g.tpr;
   g.rpb = cta_warps / warps;
-  const int64_t want = (rows + g.rpb - 1) / g.rpb;
-  g.grid = (unsigned)(want < 148 ? (want > 0 ? want : 1) : 148);
+  g.period = 1;
+  if (kind == kBnPacked)
+    while (D * g.period % kBnVec) g.period *= 2;
+  const int64_t each = (rows + g.period - 1) / g.period, want = (each + g.rpb - 1) / g.rpb, most = 148 / g.period;
+  g.grid = (unsigned)(g.period * (want < most ? (want > 0 ? want : 1) : most));
   return g;
 }
 
@@ -69,6 +89,7 @@ struct BnParams {
   KdnBlockNormArgs a;
   float* partial;  // [CTAs][2][D]: sums of dh zh and of Z s yh
   int tpr;
+  int period;
   int planes;  // 16-byte pieces of the call's inputs per vector
   int stages;  // of the ring
 };
@@ -159,11 +180,29 @@ template <> struct Raw<float> {
   __device__ __forceinline__ float2 operator[](int i) const { return make_float2(v[2 * i], v[2 * i + 1]); }
 };
 
+// 16 bytes of which at most n (0 or fewer: none) are read, zeros behind them
+__device__ __forceinline__ void cp_async16_part(void* dst, const void* src, int n) {
+  n = min(max(n, 0), 16);
+  if (n == 0) *static_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+  else
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(n)
+                 : "memory");
+}
+// values outside [lo, n) of a vector in shared memory become 0
+template <class T>
+__device__ __forceinline__ void clear_outer(const uint4* vector, int lo, int n) {
+  T* v = reinterpret_cast<T*>(const_cast<uint4*>(vector));
+#pragma unroll
+  for (int i = 0; i < kBnVec; ++i)
+    if (i < lo || i >= n) v[i] = from_f<T>(0.f);
+}
+
 // One input tensor of a call: rows of D values, `stride` apart.  The pieces of
 // a row are the 16-byte words of memory that cover it; piece 0 starts up to 15
 // bytes before the row.
-template <class T, bool ALIGNED>
+template <class T, BnRows ROWS>
 struct BnSource {
+  static constexpr bool ALIGNED = ROWS != kBnLoose;
   const char* base;
   int64_t stride;  // bytes
   int64_t rows;
@@ -191,12 +230,20 @@ struct BnSource {
   }
   // Copies this thread's pieces of row r into the ring at dst, piece after
   // piece.  Only the last slot can reach past the row's nv vectors; unaligned
-  // rows may reach one piece past them.
+  // rows may reach one piece past them.  Packed rows: from `shift` values before the row, and zeros past the tensor.
   template <int SLOTS>
-  __device__ __forceinline__ void copy(int64_t r, uint4* dst, int t, int tpr, int nv) const {
+  __device__ __forceinline__ void copy(int64_t r, uint4* dst, int t, int tpr, int nv, int shift) const {
     constexpr int P = Raw<T>::kPlanes;
-    const char* p = row(r);
-    if (ALIGNED) {
+    const char* p = row(r) - (ROWS == kBnPacked ? shift * (int)sizeof(T) : 0);
+    if (ROWS == kBnPacked && p + 16 * P * nv > base + rows * bytes) {
+      const int first = P * (t & ~31) + (t & 31), inside = (int)(base + rows * bytes - p);
+#pragma unroll 1
+      for (int s = 0; s < SLOTS; ++s)
+        for (int k = 0; k < P; ++k) {
+          const int piece = first + P * s * tpr + 32 * k;
+          if (piece < P * nv) cp_async16_part(dst + piece, p + 16 * piece, inside - 16 * piece);
+        }
+    } else if (ALIGNED) {
       // a warp's vectors of a slot are 32 P neighbouring pieces: lane by lane, so that each request is one run of memory
       const int first = P * (t & ~31) + (t & 31);
       const char* q = p + 16 * first;
@@ -272,11 +319,17 @@ __device__ __forceinline__ void words_of(uint32_t (&w)[8], const float2 (&v)[4],
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(i & 1 ? v[i / 2].y : v[i / 2].x);
 }
-template <bool ALIGNED, class T>
-__device__ __forceinline__ void put(T* p, const float2 (&v)[4], int n) {
-  if (ALIGNED) {
+template <BnRows ROWS, class T>
+__device__ __forceinline__ void put(T* p, const float2 (&v)[4], int n, int lo) {
+  if (ROWS != kBnLoose) {
     const float s[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
-    if (n > 0) st_row(p, s);
+    if (ROWS == kBnAligned ? n > 0 : lo == 0 && n == 8) {
+      st_row(p, s);
+    } else if (ROWS == kBnPacked && n > 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i >= lo && i < n) p[i] = from_f<T>(s[i]);
+    }
     return;
   }
   constexpr int W = 2 * sizeof(T);  // 32-bit words of 8 values
@@ -318,20 +371,20 @@ __device__ __forceinline__ void put(T* p, const float2 (&v)[4], int n) {
     if (i < n && !(i < 8 - e ? whole : next_whole)) p[i] = from_f<T>(i & 1 ? v[i / 2].y : v[i / 2].x);
 }
 
-// weights of 8 columns (absent: 1; past the row: 0)
-template <bool ALIGNED>
-__device__ __forceinline__ void ldw(float2 (&out)[4], const void* p, int col, int n, bool bf) {
+// weights of 8 columns, those from lo to n (absent: 1; outside the row: 0)
+template <BnRows ROWS>
+__device__ __forceinline__ void ldw(float2 (&out)[4], const void* p, int col, int n, int lo, bool bf) {
   float d[8];
   if (!p || n <= 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) d[i] = i < n ? 1.f : 0.f;
-  } else if ((ALIGNED || n == 8) && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    for (int i = 0; i < 8; ++i) d[i] = i >= lo && i < n ? 1.f : 0.f;
+  } else if ((ROWS == kBnAligned || (ROWS == kBnLoose && n == 8)) && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
     if (bf) ld8(d, static_cast<const bf16*>(p) + col);
     else ld8(d, static_cast<const float*>(p) + col);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      d[i] = i >= n ? 0.f : bf ? to_f(static_cast<const bf16*>(p)[col + i]) : static_cast<const float*>(p)[col + i];
+      d[i] = i < lo || i >= n ? 0.f : bf ? to_f(static_cast<const bf16*>(p)[col + i]) : static_cast<const float*>(p)[col + i];
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) out[i] = make_float2(d[2 * i], d[2 * i + 1]);
@@ -341,19 +394,19 @@ __device__ __forceinline__ void ldw(float2 (&out)[4], const void* p, int col, in
 // scale * post_weight next (FULL), zero at vector nv.  All row groups of a CTA share them.
 template <bool FULL>
 constexpr int kWeightPlanes = FULL ? 4 : 2;
-template <bool ALIGNED, bool FULL>
-__device__ __forceinline__ void stage_weights(float4* dst, const KdnBlockNormArgs& a, int nv) {
+template <BnRows ROWS, bool FULL>
+__device__ __forceinline__ void stage_weights(float4* dst, const KdnBlockNormArgs& a, int nv, int shift) {
   const bool wb = a.weights_bf16 != 0;
   const int plane = nv + 1;
   for (int v = threadIdx.x; v <= nv; v += blockDim.x) {
-    const int col = v * kBnVec, n = min(max((int)a.D - col, 0), kBnVec);
+    const int col = v * kBnVec - shift, n = min(max((int)a.D - col, 0), kBnVec), lo = max(-col, 0);
     float2 w[4], sc[4];
-    ldw<ALIGNED>(w, a.weight, col, n, wb);
+    ldw<ROWS>(w, a.weight, col, n, lo, wb);
     dst[v] = make_float4(w[0].x, w[0].y, w[1].x, w[1].y);
     dst[plane + v] = make_float4(w[2].x, w[2].y, w[3].x, w[3].y);
     if (!FULL) continue;
-    ldw<ALIGNED>(sc, a.scale, col, n, wb);
-    ldw<ALIGNED>(w, a.post_weight, col, n, wb);
+    ldw<ROWS>(sc, a.scale, col, n, lo, wb);
+    ldw<ROWS>(w, a.post_weight, col, n, lo, wb);
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], sc[i]);
     dst[2 * plane + v] = make_float4(w[0].x, w[0].y, w[1].x, w[1].y);
@@ -444,8 +497,9 @@ struct BnRing {
 };
 
 template <auto Kernel>
-int bn_start(BnParams p, const BnGeom& g, int weight_planes, size_t fixed, const char* what, cudaStream_t st) {
-  const size_t threads = (size_t)g.tpr * g.rpb, places = (size_t)(p.a.D + kBnVec - 1) / kBnVec + 1;
+int bn_start(BnParams p, const BnGeom& g, BnRows kind, int weight_planes, size_t fixed, const char* what,
+             cudaStream_t st) {
+  const size_t threads = (size_t)g.tpr * g.rpb, places = (size_t)bn_vectors((int)p.a.D, kind == kBnPacked) + 1;
   const size_t plane = sizeof(uint4) * places * g.rpb, weights = sizeof(float4) * weight_planes * places;
   p.stages = (int)((kBnSmem - fixed - weights) / (plane * p.planes));
   if (p.stages < 1) return set_error(KDN_ERR_INVALID, "%s: a row does not fit shared memory", what);
@@ -456,19 +510,21 @@ int bn_start(BnParams p, const BnGeom& g, int weight_planes, size_t fixed, const
   return check_launch(what);
 }
 
-// Every row of every tensor of the call starts on a 16-byte boundary (fp32
-// outputs: 32) and is a whole number of vectors (absent tensors are).
-inline bool bn_aligned(const KdnBlockNormArgs& a) {
+// Aligned: every row of every tensor of the call starts on a 16-byte boundary
+// (fp32 outputs: 32) and is a whole number of vectors (absent tensors are).
+inline BnRows bn_rows(const KdnBlockNormArgs& a) {
   const int64_t ex = a.stream_bf16 ? 2 : 4, ey = a.act_bf16 ? 2 : 4;
-  uintptr_t bits = (uintptr_t)(a.D % kBnVec);
-  for (const void* p : {a.x, a.y, a.gate, a.weight, a.post_weight, a.scale, a.dz, a.dh})
-    bits |= reinterpret_cast<uintptr_t>(p) & 15;
+  uintptr_t bits = 0, weights = 0, strides = (uintptr_t)(a.D % kBnVec);
+  for (const void* p : {a.x, a.y, a.gate, a.dz, a.dh}) bits |= reinterpret_cast<uintptr_t>(p) & 15;
+  for (const void* p : {a.weight, a.post_weight, a.scale}) weights |= reinterpret_cast<uintptr_t>(p) & 15;
   for (const void* p : {a.z, a.dx}) bits |= reinterpret_cast<uintptr_t>(p) & (8 * ex - 1);
   for (const void* p : {a.h, a.dy, a.dgate}) bits |= reinterpret_cast<uintptr_t>(p) & (8 * ey - 1);
-  bits |= (uintptr_t)(a.x_stride * ex) & 15;
-  if (a.y) bits |= (uintptr_t)(a.y_stride * ey) & 15;
-  if (a.gate) bits |= (uintptr_t)(a.gate_stride * ey) & 15;
-  return bits == 0;
+  strides |= (uintptr_t)(a.x_stride * ex) & 15;
+  if (a.y) strides |= (uintptr_t)(a.y_stride * ey) & 15;
+  if (a.gate) strides |= (uintptr_t)(a.gate_stride * ey) & 15;
+  if ((bits | weights | strides) == 0) return kBnAligned;
+  const bool packed = a.x_stride == a.D && (!a.y || a.y_stride == a.D) && (!a.gate || a.gate_stride == a.D);
+  return bits == 0 && packed ? kBnPacked : kBnLoose;
 }
 
 }  // namespace

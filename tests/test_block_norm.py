@@ -292,3 +292,27 @@ def test_c_entry_refuses_without_launch():
     a.dscale = 16
     assert lib.kdn_block_norm_bwd(a, None) == -1 and b"absent input" in lib.kdn_last_error()
     assert lib.kdn_block_norm_workspace_bytes(4, 32) > 0 and lib.kdn_block_norm_workspace_bytes(0, 32) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [3, 36, 97, 1155])
+@pytest.mark.parametrize("stream,dtype", [(BF, BF), (F, F)])
+def test_rows_do_not_touch_their_neighbours(D, stream, dtype):
+    """Rows that share 16-byte words of memory: what one of them holds changes nothing in the others, and an output
+    row ends where the next begins."""
+    d = make((21, D), stream, dtype, "ypgs", seed=D)
+    z, h, grads = ours(d)
+    for k in ("x", "y", "gate", "dz", "dh"):
+        d[k] = d[k].clone()
+        d[k][7], d[k][12] = float("nan"), float("inf")
+    zn, hn, spoilt = ours(d)
+    rest = [i for i in range(21) if i not in (7, 12)]
+    for a, b in ((z, zn), (h, hn), *((grads[k], spoilt[k]) for k in ("x", "y", "gate"))):
+        assert torch.equal(a[rest], b[rest]) and not b[7].isfinite().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 9, 1201])
+@pytest.mark.parametrize("D", [10, 100, 801])
+def test_few_and_many_odd_rows(rows, D):
+    compare(make((rows, D), F, F, "ypgs", seed=rows + D))
