@@ -16,13 +16,15 @@
 // dpost share one sum, sum Z s yh, because the weights are factors of whole
 // columns.  The coming rows are copied into a ring in shared memory
 // (cp.async), which keeps enough bytes in flight without holding registers.
-// Rows that do not start on 16-byte boundaries are copied as the aligned
-// pieces that cover them and shifted when they are read.  The groups' sums are
+// Rows of odd widths in contiguous tensors are worked on as the aligned words
+// that cover them, rows of other strides and alignments are copied so and
+// shifted when they are read (BnRows).  The groups' sums are
 // added in a fixed order by a second kernel.
 //
-// 16384 x 2304 bf16: all parts 68 us forward (5.5 TB/s) and 116 us backward
-// (5.2 TB/s, the second kernel included), the plain sum 55 and 87 us; with an
-// fp32 stream 99 / 153 and 84 / 126 us.
+// 16384 x 2304 bf16: all parts 68 us forward (5.5 TB/s) and 114 us backward
+// (5.3 TB/s, the second kernel included), the plain sum 55 and 88 us; with an
+// fp32 stream 99 / 153 and 85 / 126 us.  8192 x 2304 bf16 39 / 67, 8192 x 2305
+// 57 / 97 (four warps a row instead of three, and the outer vectors).
 #pragma once
 
 #include "kdn_launch.cuh"
@@ -35,13 +37,13 @@ constexpr int kBnMaxD = 8192;
 constexpr int kBnMinD = 2;  // the norm of one value is its sign: fp32 cannot resolve its gradient (of the order of eps)
 // A row belongs to the fewest warps whose lanes hold it in three slots each:
 // what a row costs beside its values (reductions, addresses, barriers) is paid
-// per warp.  The backward of unaligned rows (dense false) takes as few slots as
-// the CTA's warps allow instead: every slot's shifts are code of its own, more
-// of it than registers and instruction fetch bear (1000 x 1155 fp32: 31 us
-// against 39; 8192 x 2305 bf16: 203 against 218; the forward loses, 125 us
-// against 79).  One CTA per SM with as many rows at a time as its
-// warps make: 12 warps (168 registers a thread), in the forward of unaligned
-// rows, which wait at a barrier per row, 16.
+// per warp.  The backward of loose rows (see BnRows) takes as few slots as the
+// CTA's warps allow instead: every slot's shifts are code of its own, more of it
+// than registers and instruction fetch bear (rows of 1155 fp32 values, 1000 of
+// them: 31 us against 39; 8192 of 2305 bf16: 203 against 218; the forward loses,
+// 125 us against 79).  One CTA per SM with as many rows at a time as its warps
+// make: 12 warps (168 registers a thread), in the forward of loose rows, which
+// wait at a barrier per row, 16.
 constexpr int kBnFwdWarps = 16, kBnBwdWarps = 12, kBnSlots = 3;
 constexpr size_t kBnSmem = 232448;  // a CTA's shared memory; fp32 rows of 8192 values and their weights fit once
 
@@ -61,7 +63,10 @@ struct BnGeom {
 // rows of one shift only, so that its weights and its columns' sums are those of
 // aligned rows, moved by it; only the outer vectors of a row differ (what they
 // hold of the neighbours is cleared in shared memory, their values are stored
-// one by one).  Loose: any other strides and alignments.
+// one by one).  Loose: any other strides and alignments, every vector shifted
+// when it is read and when it is stored.  8192 x 2305 bf16, all parts: packed 57
+// us forward and 97 backward, loose 80 and 204; 1000 x 1155 fp32: 12.5 and 25,
+// loose 12.5 and 31.
 enum BnRows { kBnLoose = 0, kBnAligned = 1, kBnPacked = 2 };
 
 // vectors of a row (packed: of the rows with the largest shift)
