@@ -111,7 +111,8 @@ struct Chunk {
     }
     cp_async_commit();
   }
-  // f(logits, first index, how many) for this thread's groups, in a fixed order (past the end: -inf)
+  // f(logits, first index) for this thread's groups, in a fixed order (past the end: -inf).  first index: begin and a
+  // multiple of kPer
   template <class F>
   __device__ __forceinline__ void each(F&& f) const {
 #pragma unroll 1
@@ -131,15 +132,19 @@ struct Chunk {
         for (int k = 0; k < kPer; ++k) v[k] = fminf(v[k], kLargest);
       f(v, first(j));
     }
-    const int done = groups * kSmThreads * kPer;
+    // what does not fit: further groups of the same shape, so that f meets the same alignments
 #pragma unroll 1
-    for (int j = 0; begin + done + j * kSmThreads < end; ++j) {
-      const int i = begin + done + j * kSmThreads + (int)threadIdx.x;
+    for (int i = first(groups); i < end; i += kSmThreads * kPer) {
       float v[kPer];
+      if (VEC && i + kPer <= end) {
+        if constexpr (VEC) ld8(v, row + i);
+      } else {
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) v[k] = -INFINITY;
-      if (i < end) v[0] = to_f(row[i]);
-      if (infinite) v[0] = fminf(v[0], kLargest);
+        for (int k = 0; k < kPer; ++k) v[k] = i + k < end ? to_f(row[i + k]) : -INFINITY;
+      }
+      if (infinite)
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) v[k] = fminf(v[k], kLargest);
       f(v, i);
     }
   }
@@ -260,7 +265,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const __grid_cons
   const float scale = __fdiv_rd(1.4426950408889634f, temp);
   const float rest = fmaxf(fmaf(-scale, temp, 1.4426950408889634f) / temp, 1e-30f);
   auto weight = [&](float l) { return fmaxf(ex2a(-fmaf(top - l, scale, (top - l) * rest)), 0.f); };  // NaN: 0
-  // the random numbers of a group: one 32-byte sector, in one round trip
+  // the random numbers of a group: one 32-byte sector, in one round trip (VEC: begin, and with it i, is a multiple of 8)
   const bool noise16 = (reinterpret_cast<uintptr_t>(E) & 15) == 0;
   auto draw = [&](float (&noise)[PER], int i) {
     if (PER == 8 && noise16 && i + 8 <= c.end) {

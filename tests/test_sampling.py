@@ -262,3 +262,28 @@ def test_c_entry_refuses_without_launch():
     a.logits = a.noise = a.token = a.prob = 16
     a.logits_stride = 9
     assert lib.kdn_sample(a, None) == -1 and b"strides" in lib.kdn_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 800000), (torch.bfloat16, 786433), (torch.float32, 400003)])
+@pytest.mark.parametrize("options", [{}, {"top_k": 1}, {"top_k": 2000}, {"top_p": 0.6}, {"temperature": 0.0},
+                                     {"top_k": 300, "top_p": 0.9, "min_p": 0.001}])
+def test_rows_beyond_shared_memory(dtype, V, options):
+    """Vocabularies of which eight CTAs of 192 KB do not hold a row: the rest is read again in every pass.  Winners and
+    kept tokens among that rest, rows that start on 16-byte boundaries and rows that do not."""
+    held, chunk = 192 * 1024 // dtype.itemsize, (V + 63) // 64 * 8
+    rest = torch.arange(V) % chunk >= held
+    assert rest.any()
+    wide, wide_n = V + 8 - V % 8 + 8, V + 4 - V % 4 + 4  # row strides of whole 16-byte words
+    logits, noise = make(3, V, dtype, 2.0, seed=V)
+    logits[1, rest] += 6.0
+    logits[2, ~rest] = -math.inf
+    want, _ = check(logits, noise, **options)
+    assert rest[want[2]]
+    for shift in (0, 3):
+        l = torch.full((3, wide), 50.0, dtype=dtype, device="cuda")
+        n = torch.full((3, wide_n), 1e-9, device="cuda")
+        l[:, shift:shift + V], n[:, shift:shift + V] = logits.cuda(), noise.cuda()
+        for i in (slice(None), slice(1, 2)):
+            token, _ = sample(l[i, shift:shift + V], n[i, shift:shift + V], **options)
+            assert torch.equal(token.cpu(), want[i])
