@@ -83,6 +83,8 @@ struct Chunk {
   bool infinite = false;    // +inf is among the row's logits: it counts as the largest finite value
   T* held;
 
+  // +inf becomes the largest finite value; NaN stays (fminf would make it a number)
+  __device__ __forceinline__ static float finite(float v) { return v > kLargest ? kLargest : v; }
   __device__ __forceinline__ int first(int j) const { return begin + (j * kSmThreads + (int)threadIdx.x) * kPer; }
   // place of this thread's group j; fp32 vectors are split over two planes
   __device__ __forceinline__ T* place(int j) const {
@@ -129,7 +131,7 @@ struct Chunk {
       }
       if (infinite)
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) v[k] = fminf(v[k], kLargest);
+        for (int k = 0; k < kPer; ++k) v[k] = finite(v[k]);
       f(v, first(j));
     }
     // what does not fit: further groups of the same shape, so that f meets the same alignments
@@ -144,7 +146,7 @@ struct Chunk {
       }
       if (infinite)
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) v[k] = fminf(v[k], kLargest);
+        for (int k = 0; k < kPer; ++k) v[k] = finite(v[k]);
       f(v, i);
     }
   }

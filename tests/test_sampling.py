@@ -287,3 +287,18 @@ def test_rows_beyond_shared_memory(dtype, V, options):
         for i in (slice(None), slice(1, 2)):
             token, _ = sample(l[i, shift:shift + V], n[i, shift:shift + V], **options)
             assert torch.equal(token.cpu(), want[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [700, 1501, 40000])
+@pytest.mark.parametrize("options", [{"temperature": 0.0}, {}, {"top_k": 3}, {"top_p": 0.6}, {"min_p": 0.5}])
+def test_nan_beside_infinity(dtype, V, options):
+    """NaN logits count as -inf in rows with +inf too, whichever comes first."""
+    logits, noise = make(3, V, dtype, seed=V)
+    logits[:, ::3] = math.nan
+    logits[0, [1, 640]] = math.inf
+    logits[1, [4, 5, 695]] = math.inf
+    logits[2, 698] = math.inf
+    token, _ = check(logits, noise, **options)
+    assert token[2] == 698
