@@ -263,10 +263,11 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const __grid_cons
   if (c.infinite) top = kLargest, floor_l = fminf(floor_l, kLargest);
 
   // ---- 2: Z, and the histogram or the only race ----
-  // e = 2^-t, t = (top - l) log2(e) / T in two terms; both are positive, so that -inf gives t = inf, e = 0
+  // e = 2^-t, t = (top - l) log2(e) / T in two terms, neither negative (T = inf: both 0, an even draw); -inf gives t = inf
+  // or, where a term is 0, NaN: e = 0 both ways
   const float scale = __fdiv_rd(1.4426950408889634f, temp);
-  const float rest = fmaxf(fmaf(-scale, temp, 1.4426950408889634f) / temp, 1e-30f);
-  auto weight = [&](float l) { return fmaxf(ex2a(-fmaf(top - l, scale, (top - l) * rest)), 0.f); };  // NaN: 0
+  const float rest = fmaxf(fmaf(-scale, temp, 1.4426950408889634f) / temp, 0.f);
+  auto weight = [&](float l) { return fmaxf(ex2a(-fmaf(top - l, scale, (top - l) * rest)), 0.f); };
   // the random numbers of a group: one 32-byte sector, in one round trip (VEC: begin, and with it i, is a multiple of 8)
   const bool noise16 = (reinterpret_cast<uintptr_t>(E) & 15) == 0;
   auto draw = [&](float (&noise)[PER], int i) {

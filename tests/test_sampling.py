@@ -302,3 +302,29 @@ def test_nan_beside_infinity(dtype, V, options):
     logits[2, 698] = math.inf
     token, _ = check(logits, noise, **options)
     assert token[2] == 698
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1e20, 1e32, math.inf])
+@pytest.mark.parametrize("options", [{}, {"top_k": 9}, {"top_p": 0.4937}])
+def test_hot_rows(T, options):
+    """Temperatures beside which the logits' differences are small, whatever their size: finite masks and large logits
+    are drawn with their weight, -inf never."""
+    logits, noise = make(8, 900, torch.float32, seed=4)
+    logits[:, ::2] = torch.finfo(torch.float32).min
+    logits[1] = logits[1].clamp(-1, 1) * 1e32
+    logits[2] = -math.inf
+    logits[2, 100:] = -1e31
+    logits[3, 5::7] = -math.inf
+    token, prob = sample(logits.cuda(), noise.cuda(), temperature=T, **options)
+    unclear = 0
+    for i in range(8):  # the definition over the tokens above -inf: exp(-inf / T) is 0, also where T is infinite
+        at = torch.nonzero(logits[i] > -math.inf)[:, 0]
+        want, p, clear = truth(logits[i, at].numpy(), noise[i, at].numpy(), T, options.get("top_k"), options.get("top_p"),
+                               None)
+        if not clear:
+            unclear += 1
+            continue
+        assert token[i].item() == at[want], i
+        assert abs(prob[i].item() - p) <= 1e-5 * p, i
+    assert unclear <= 1
