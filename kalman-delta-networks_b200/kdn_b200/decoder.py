@@ -164,7 +164,7 @@ class KDNDecoder(nn.Module):
     @torch.no_grad()
     def generate(self, prompts, count, *, generator=None, graph=True, **options):
         """``count`` tokens after every row of prompts [B, T]; options as :func:`~kdn_b200.sampling.sample` takes them.
-        Returns (tokens [B, count], their probabilities [B, count])."""
+        Returns (tokens [B, count], their probabilities [B, count]); -1 and 0 where a row's logits are all NaN or -inf."""
         B = prompts.shape[0]
         pools, steps = self.make_pools(B), [m.make_step() for m in self.mixers]
         slots = torch.arange(B, dtype=torch.int32, device=prompts.device)
@@ -172,8 +172,9 @@ class KDNDecoder(nn.Module):
         noise = torch.empty(B, self.vocab, device=prompts.device)
         draw = lambda: noise.exponential_(generator=generator).clamp_(min=1e-30)  # noqa: E731
         draw()
-        token, prob = sample(logits, noise, **options)
-        tokens, probs = [token.clone()], [prob.clone()]
+        new, prob = sample(logits, noise, **options)
+        tokens, probs = [new.clone()], [prob.clone()]
+        token = new.clamp(min=0)  # a row that lost its numbers (token -1) goes on with token 0: the embedding has no row -1
 
         def advance():
             return sample(self.decode(token, pools, steps, slots), noise, **options)
@@ -189,7 +190,7 @@ class KDNDecoder(nn.Module):
                     with torch.cuda.graph(replay):  # records only
                         new, p = advance()
                 replay.replay()
-            token.copy_(new)
+            torch.clamp(new, min=0, out=token)
             tokens.append(new.clone())
             probs.append(p.clone())
         return torch.stack(tokens, 1), torch.stack(probs, 1)

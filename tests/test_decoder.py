@@ -77,3 +77,16 @@ def test_trains(variant):
 def test_refuses_unknown_variants():
     with pytest.raises(ValueError, match="variant"):
         KDNDecoder(16, 128, 1, 1, variant="other", device="cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("variant", ["iso", "diag"])
+def test_rows_without_a_token_go_on(variant):
+    """Logits that are all NaN give token -1, which must not reach the embedding."""
+    model = make(variant, seed=5)
+    prompts = torch.randint(VOCAB, (3, 9), device="cuda")
+    with torch.no_grad():
+        model.head.weight.fill_(float("nan"))
+    for graph in (True, False):
+        tokens, probs = model.generate(prompts, 6, graph=graph, top_k=3)
+        assert tokens.shape == (3, 6) and (tokens == -1).all() and (probs == 0).all()
