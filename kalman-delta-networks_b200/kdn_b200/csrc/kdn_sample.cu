@@ -83,8 +83,12 @@ struct Chunk {
   bool infinite = false;    // +inf is among the row's logits: it counts as the largest finite value
   T* held;
 
-  // +inf becomes the largest finite value; NaN stays (fminf would make it a number)
-  __device__ __forceinline__ static float finite(float v) { return v > kLargest ? kLargest : v; }
+  // +inf becomes the largest finite value; NaN stays NaN (fminf would return the number beside it)
+  __device__ __forceinline__ static float finite(float v) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(v), "f"(kLargest));
+    return d;
+  }
   __device__ __forceinline__ int first(int j) const { return begin + (j * kSmThreads + (int)threadIdx.x) * kPer; }
   // place of this thread's group j; fp32 vectors are split over two planes
   __device__ __forceinline__ T* place(int j) const {
