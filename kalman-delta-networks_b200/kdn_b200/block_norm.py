@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -139,7 +140,7 @@ def block_norm(x, y, weight, *, post_weight=None, gate=None, scale=None, alpha=1
     x [..., D] bf16 or fp32; y and gate [..., D] in x's dtype, or bf16 beside an fp32 x; weight, post_weight and scale [D]
     (one dtype, bf16 or fp32).  ``post_weight`` None: no norm after the block; ``gate`` None: no gate; ``scale`` None: 1.
     ``alpha`` is a Python number multiplying x.  z has x's dtype, h has y's.  With ``y`` None (before the first block) z
-    is x itself and h = norm(x) * weight.  Differentiable in every tensor.
+    is x itself and h = norm(x) * weight.  Differentiable in every tensor, once and in reverse mode.
     """
     alpha, eps = float(alpha), float(eps)
     fast = N.host()
@@ -154,8 +155,10 @@ def block_norm(x, y, weight, *, post_weight=None, gate=None, scale=None, alpha=1
     x2 = _rows(x, D)
     y2 = None if y is None else _rows(y, D)
     g2 = None if gate is None else _rows(gate, D)
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad
-                                        for t in (x, y, gate, weight, post_weight, scale)]):
+    leaves = [t for t in (x, y, gate, weight, post_weight, scale) if t is not None]
+    # forward-mode tangents go to the function too: it refuses them (no jvp) instead of dropping them
+    if (torch.is_grad_enabled() and any([t.requires_grad for t in leaves])) or any(
+            [forward_ad.unpack_dual(t).tangent is not None for t in leaves]):
         weight, post_weight, scale = [None if w is None else w.contiguous() for w in (weight, post_weight, scale)]
         z, h = _BlockNormFunction.apply(x2, y2, g2, weight, post_weight, scale, alpha, swish, eps)
         if y is None and not x.requires_grad:

@@ -49,6 +49,8 @@ void launch(int (*fn)(const Args*, kdn_stream_t), const Args& args, const Tensor
 
 bool is_bf16(const Tensor& t) { return t.scalar_type() == at::kBFloat16; }
 bool is_float(const Tensor& t) { return is_bf16(t) || t.scalar_type() == at::kFloat; }
+// carries a forward-mode tangent, which no operator here propagates: the Python path refuses it
+bool is_dual(const Tensor& t) { return t._fw_grad(0).defined(); }
 const void* ptr(const Optional& t) { return t ? t->const_data_ptr() : nullptr; }
 
 // rows [B, width] of a type and device, their values contiguous
@@ -227,9 +229,10 @@ std::optional<std::tuple<Tensor, Tensor>> block_norm(const Tensor& x, const Tens
   const int64_t D = x.size(-1);
   if (D < least || D > most || x.numel() == 0) return std::nullopt;
   if (is_bf16(x) && !is_bf16(y)) return std::nullopt;
-  if (gate && (gate->sizes() != x.sizes() || gate->scalar_type() != y.scalar_type())) return std::nullopt;
+  if (is_dual(x) || is_dual(y)) return std::nullopt;
+  if (gate && (is_dual(*gate) || gate->sizes() != x.sizes() || gate->scalar_type() != y.scalar_type())) return std::nullopt;
   for (const Tensor* w : {&weight, post_weight ? &*post_weight : nullptr, scale ? &*scale : nullptr})
-    if (w && (w->dim() != 1 || w->size(0) != D || !w->is_contiguous() || !is_float(*w) ||
+    if (w && (is_dual(*w) || w->dim() != 1 || w->size(0) != D || !w->is_contiguous() || !is_float(*w) ||
               w->scalar_type() != weight.scalar_type() || w->device() != x.device()))
       return std::nullopt;
   for (const Tensor* t : {&x, &y, gate ? &*gate : nullptr})

@@ -150,3 +150,25 @@ def test_refusals_are_the_same():
                 call()
             errors.append((e.type, str(e.value)))
         assert errors[0] == errors[1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", [contextlib.nullcontext, python_path])
+@pytest.mark.parametrize("which", ["x", "y", "weight", "post_weight", "gate", "scale"])
+@pytest.mark.parametrize("grad", [True, False])
+def test_block_norm_refuses_forward_mode_derivatives(path, which, grad):
+    from torch.autograd import forward_ad
+
+    args = {k: torch.randn(*((5, 40) if k in ("x", "y", "gate") else (40,)), device="cuda")
+            for k in ("x", "y", "weight", "post_weight", "gate", "scale")}
+    with path(), torch.set_grad_enabled(grad), forward_ad.dual_level():
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            block_norm(**args)
+        if which in ("x", "weight"):  # without a block
+            with pytest.raises(NotImplementedError, match="jvp"):
+                block_norm(args["x"], None, args["weight"])
+    with path(), forward_ad.dual_level():  # a level without tangents changes nothing
+        plain = {k: forward_ad.unpack_dual(v).primal for k, v in args.items()}
+        z, _ = block_norm(**plain)
+    assert torch.equal(z, block_norm(**plain)[0])
