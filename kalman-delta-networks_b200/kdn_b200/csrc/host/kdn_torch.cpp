@@ -50,7 +50,7 @@ void launch(int (*fn)(const Args*, kdn_stream_t), const Args& args, const Tensor
 bool is_bf16(const Tensor& t) { return t.scalar_type() == at::kBFloat16; }
 bool is_float(const Tensor& t) { return is_bf16(t) || t.scalar_type() == at::kFloat; }
 // carries a forward-mode tangent, which no operator here propagates: the Python path refuses it
-bool is_dual(const Tensor& t) { return t._fw_grad(0).defined(); }
+bool is_dual(const Tensor& t) { return t.unsafeGetTensorImpl()->autograd_meta() && t._fw_grad(0).defined(); }
 const void* ptr(const Optional& t) { return t ? t->const_data_ptr() : nullptr; }
 
 // rows [B, width] of a type and device, their values contiguous
@@ -74,6 +74,10 @@ std::optional<Tensor> step(const std::string& args, const Tensor& memory, const 
   if (!rows_of(qkv, B, 3 * channels, qkv) || !rows_of(decay, B, channels, qkv) || !rows_of(gate, B, channels, qkv) ||
       !rows_of(omega, B, iso ? 2 * a.H : channels, qkv) || (!iso && (!r || !rows_of(*r, B, a.H, qkv))))
     return std::nullopt;
+  // the Python path says that the step has no derivative
+  const bool grad = at::GradMode::is_enabled();
+  for (const Tensor* t : {&qkv, &decay, &omega, iso ? nullptr : &*r, &gate})
+    if (t && t->unsafeGetTensorImpl()->autograd_meta() && ((grad && t->requires_grad()) || is_dual(*t))) return std::nullopt;
   if (window.scalar_type() != qkv.scalar_type() || memory.device() != qkv.device()) return std::nullopt;
   if (slots) {
     if (slots->dim() != 1 || slots->size(0) != B || !slots->is_contiguous() || slots->device() != qkv.device() ||

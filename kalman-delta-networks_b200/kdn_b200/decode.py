@@ -15,6 +15,10 @@ and the gated output norm.
 The arithmetic is fp32 throughout: the convolution's outputs, the normalised
 q and k and the readout, which the training path rounds to bf16 between its
 kernels, are not rounded here.
+
+The step serves and has no derivative: parameters are taken detached, and in
+grad mode an output of inputs that require gradients raises when its backward
+is asked for (forward-mode tangents are refused at once).
 """
 from __future__ import annotations
 
@@ -22,6 +26,7 @@ import math
 from numbers import Real
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 from .norm_gated import _ACTIVATIONS
@@ -124,6 +129,18 @@ def _finite(name, value):
     return float(value)
 
 
+class _StepFunction(torch.autograd.Function):
+    """A step on inputs that require gradients: an error where one is asked for, not a graph that ends in silence."""
+
+    @staticmethod
+    def forward(ctx, launch, *inputs):
+        return launch()
+
+    @staticmethod
+    def backward(ctx, dy):
+        raise RuntimeError("kdn_b200 step: the token step has no gradient (train on the chunked operators)")
+
+
 class _Step:
     """The parameters of one mixer laid out for ``kdn_step`` (fp32 copies where
     they are not fp32 already: make a new step after changing parameters)."""
@@ -203,13 +220,22 @@ class _Step:
             raise ValueError("all step tensors must share one CUDA device")
         if not qkv.is_cuda:
             N.require_cuda(qkv)
+        inputs = (qkv, *(t for _, t, _ in rows))
+        if any([forward_ad.unpack_dual(t).tangent is not None for t in inputs]):
+            raise NotImplementedError("kdn_b200 step: the token step has no jvp (forward-mode derivative)")
+        if torch.is_grad_enabled() and any([t.requires_grad for t in inputs]):
+            return _StepFunction.apply(lambda: self._launch(state, slots, *inputs), *inputs)
+        return self._launch(state, slots, *inputs)
+
+    def _launch(self, state, slots, qkv, *rows):
         lib = N.load_library()
-        y = qkv.new_empty((B, channels))
+        B = qkv.shape[0]
+        y = qkv.new_empty((B, self.num_heads * self.head_dim))
         a = N.KdnStepArgs.from_buffer_copy(self._args)
-        a.act_bf16 = dtype == torch.bfloat16
+        a.act_bf16 = qkv.dtype == torch.bfloat16
         a.B, a.num_slots = B, state.num_slots
         a.qkv, a.qkv_stride = qkv.data_ptr(), qkv.stride(0)
-        self._rows(a, *(t for _, t, _ in rows))
+        self._rows(a, *rows)
         if slots is not None:
             a.slots, a.slots_i64 = slots.data_ptr(), slots.dtype == torch.int64
         a.memory, a.covariance = state.memory.data_ptr(), state.covariance.data_ptr()

@@ -172,3 +172,45 @@ def test_block_norm_refuses_forward_mode_derivatives(path, which, grad):
         plain = {k: forward_ad.unpack_dual(v).primal for k, v in args.items()}
         z, _ = block_norm(**plain)
     assert torch.equal(z, block_norm(**plain)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", [contextlib.nullcontext, python_path])
+@pytest.mark.parametrize("variant,which", [("iso", i) for i in range(4)] + [("diag", i) for i in range(5)])
+def test_step_says_that_it_has_no_derivative(path, variant, which):
+    from torch.autograd import forward_ad
+
+    B, H, D = 2, 2, 64
+    gen = torch.Generator().manual_seed(7)
+    n = lambda *s: torch.randn(*s, generator=gen).cuda()  # noqa: E731
+    shared = dict(conv_weight=n(3 * H * D, 4).requires_grad_(True), A_log=n(H), dt_bias=n(H * D), norm_weight=n(D))
+    if variant == "iso":
+        step = IsoKDNStep(**shared, omega_bias=n(H), r_bias=n(H), omega_min=0.0, r_min=0.01)
+        widths = (3 * H * D, H * D, 2 * H, H * D)
+    else:
+        step = DiagKDNStep(**shared)
+        widths = (3 * H * D, H * D, H * D, H, H * D)
+    token = [n(B, w) for w in widths]
+
+    def run():
+        state = KDNState.allocate(variant, B, H, D, dtype=torch.float32)
+        state.reset(slice(None), torch.ones(H, device="cuda"))
+        return step(state, *token)
+
+    with path():
+        want = run()
+        assert not want.requires_grad
+        token[which].requires_grad_(True)
+        y = run()
+        assert torch.equal(y, want)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            y.sum().backward()
+        with torch.no_grad():
+            y = run()
+        assert torch.equal(y, want) and not y.requires_grad
+        with torch.no_grad(), forward_ad.dual_level():
+            token[which] = forward_ad.make_dual(token[which].detach(), torch.ones_like(token[which]))
+            state = KDNState.allocate(variant, B, H, D, dtype=torch.float32)
+            with pytest.raises(NotImplementedError, match="jvp"):
+                step(state, *token)
+            assert not state.window.any()  # refused before anything has happened
