@@ -263,7 +263,9 @@ struct BnSource {
     } else {
       const int end = lead(p) + bytes;
       const char* q = p - lead(p);
-      const bool inner = r > 0 && r < rows - 1;  // rows whose outer pieces lie inside the tensor
+      // rows whose outer pieces lie inside the tensor: less than 16 bytes outside the row, where its neighbours' starts are
+      // 16 or more away (not so with one row for all, stride 0, or rows of a few values)
+      const bool inner = stride >= 16 && r > 0 && r < rows - 1;
 #pragma unroll
       for (int s = 0; s < P * SLOTS + 1; ++s) {
         const int piece = t + s * tpr;

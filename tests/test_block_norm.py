@@ -316,3 +316,48 @@ def test_rows_do_not_touch_their_neighbours(D, stream, dtype):
 @pytest.mark.parametrize("D", [10, 100, 801])
 def test_few_and_many_odd_rows(rows, D):
     compare(make((rows, D), F, F, "ypgs", seed=rows + D))
+
+
+def loose(t, offset=1, gap=2):
+    """t's rows as slices of wider ones, `offset` values behind a 16-byte boundary, NaN around them."""
+    wide = torch.full((t.shape[0], t.shape[1] + offset + gap), float("nan"), dtype=t.dtype, device=t.device)
+    view = wide[:, offset:offset + t.shape[1]]
+    view.copy_(t)
+    return view
+
+
+def check_loose(d, lay, **kw):
+    """Outputs and every gradient against the formula; lay: how a CPU tensor [rows, D] goes to the GPU."""
+    leaves = {}
+    for k in NAMES:
+        if d[k] is not None:
+            leaves[k] = (lay(k, d[k]) if d[k].ndim == 2 else d[k].cuda()).detach().requires_grad_(True)
+    get = leaves.get
+    z, h = block_norm(get("x"), get("y"), get("weight"), post_weight=get("post_weight"), gate=get("gate"),
+                      scale=get("scale"), **kw)
+    zr, hr, gr = reference(d, **kw)
+    assert nmax(z, zr) < tol_of(z) and nmax(h, hr) < tol_of(h)
+    grads = torch.autograd.grad((z, h), list(leaves.values()), (d["dz"].cuda(), d["dh"].cuda()))
+    for k, g in zip(leaves, grads):
+        assert g.dtype == d[k].dtype and g.shape == d[k].shape
+        assert nmax(g, gr[k]) < tol_of(g, k in NAMES[3:]), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [2, 3, 5, 7])
+@pytest.mark.parametrize("stream,dtype", [(BF, BF), (F, BF), (F, F)])
+def test_narrow_strides(D, stream, dtype):
+    """Rows that start less than 16 bytes apart: the words that cover a row reach past its neighbours."""
+    check_loose(make((37, D), stream, dtype, "ypgs", seed=D), lambda k, t: loose(t.cuda(), 1, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [3, 97, 1155])
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("offset", [0, 1, 5])
+def test_one_odd_row_for_all(D, dtype, offset):
+    """Stride 0 at odd widths and offsets, NaN on both sides of the one row."""
+    d = make((11, D), dtype, dtype, "ypgs", seed=D + offset)
+    for k in ("x", "gate"):
+        d[k] = d[k][:1].expand(11, D)
+    check_loose(d, lambda k, t: loose(t[:1].cuda(), offset).expand(11, D) if k in ("x", "gate") else t.cuda())
