@@ -361,3 +361,33 @@ def test_one_odd_row_for_all(D, dtype, offset):
     for k in ("x", "gate"):
         d[k] = d[k][:1].expand(11, D)
     check_loose(d, lambda k, t: loose(t[:1].cuda(), offset).expand(11, D) if k in ("x", "gate") else t.cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,many", [(3, 8000), (97, 8000), (1155, 5000), (4099, 700), (8191, 700)])
+@pytest.mark.parametrize("stream,dtype", [(BF, BF), (F, BF), (F, F)])
+@pytest.mark.parametrize("parts,few", [("y", True), ("ypgs", True), ("ypgs", False), ("pygs", False)])
+def test_loose_rows_match_formula(D, many, stream, dtype, parts, few):
+    """Outputs and gradients of rows with odd strides and offsets (cotangents too): few, and more than the CTAs hold at a
+    time.  Weight gradients: the sums of up to 8000 random terms have partial sums of the order of the result, added in
+    some 50 steps, 50 * 2^-24 = 3e-6 of it: 2e-5."""
+    rows = 5 if few else many
+    offsets = {"x": 1, "y": 3, "gate": 2} if parts == "ypgs" else {"x": 0, "y": 1, "gate": 7}
+    d = make((rows, D), stream, dtype, parts, seed=D + rows)
+    leaves = {k: None if d[k] is None else (loose(d[k].cuda(), offsets[k]) if k in offsets else d[k].cuda())
+              .detach().requires_grad_(True) for k in NAMES}
+
+    def packed(t):  # contiguous, one value behind a 16-byte boundary
+        room = torch.full((t.numel() + 1,), float("nan"), dtype=t.dtype, device="cuda")
+        room[1:] = t.cuda().flatten()
+        return room[1:].view(t.shape)
+
+    z, h = block_norm(leaves["x"], leaves["y"], leaves["weight"], post_weight=leaves["post_weight"], gate=leaves["gate"],
+                      scale=leaves["scale"])
+    zr, hr, gr = reference(d)
+    assert nmax(z, zr) < tol_of(z) and nmax(h, hr) < tol_of(h)
+    names = [k for k in NAMES if leaves[k] is not None]
+    grads = torch.autograd.grad((z, h), [leaves[k] for k in names], (packed(d["dz"]), packed(d["dh"])))
+    for k, g in zip(names, grads):
+        assert g.dtype == d[k].dtype and g.shape == d[k].shape
+        assert nmax(g, gr[k]) < tol_of(g, k in NAMES[3:]), k
