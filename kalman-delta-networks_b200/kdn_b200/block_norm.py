@@ -29,11 +29,12 @@ _DTYPES = (torch.bfloat16, torch.float32)
 
 
 def _rows(t, D):
-    """[..., D] as [rows, D] with contiguous rows (a view where the strides allow one).  ``empty_like`` of it is
-    contiguous, whatever the rows' stride."""
+    """[..., D] as [rows, D] with contiguous rows that do not overlap, or one row for all (a view where the strides allow
+    one).  ``empty_like`` of it is contiguous, whatever the rows' stride."""
     if t.ndim != 2:
         t = t.reshape(-1, D)
-    return t if t.stride(1) == 1 else t.contiguous()
+    apart = t.shape[0] <= 1 or t.stride(0) >= D or t.stride(0) == 0
+    return t if apart and t.stride(1) == 1 else t.contiguous()
 
 
 def _args(x, y, gate, weight, post_weight, scale, z, h, rstd, alpha, swish, eps):

@@ -224,7 +224,12 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
   }
 };
 
-// rows [rows, D] with contiguous values; the gate and the block's output as x
+// [rows, D] with contiguous rows that do not overlap, or one row for all
+bool apart(const Tensor& t) {
+  return t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) >= t.size(1) || t.stride(0) == 0);
+}
+
+// rows [rows, D] as apart() wants them; the gate and the block's output as x
 std::optional<std::tuple<Tensor, Tensor>> block_norm(const Tensor& x, const Tensor& y, const Tensor& weight,
                                                      const Optional& post_weight, const Optional& gate,
                                                      const Optional& scale, double alpha, int64_t swish, double eps,
@@ -240,7 +245,7 @@ std::optional<std::tuple<Tensor, Tensor>> block_norm(const Tensor& x, const Tens
               w->scalar_type() != weight.scalar_type() || w->device() != x.device()))
       return std::nullopt;
   for (const Tensor* t : {&x, &y, gate ? &*gate : nullptr})
-    if (t && (t->device() != x.device() || (t->dim() == 2 ? t->stride(1) != 1 : !t->is_contiguous()))) return std::nullopt;
+    if (t && (t->device() != x.device() || (t->dim() == 2 ? !apart(*t) : !t->is_contiguous()))) return std::nullopt;
   const bool flat = x.dim() == 2;
   const Tensor x2 = flat ? x : x.view({-1, D}), y2 = flat ? y : y.view({-1, D});
   const Optional g2 = !gate || flat ? gate : Optional(gate->view({-1, D}));

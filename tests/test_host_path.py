@@ -214,3 +214,24 @@ def test_step_says_that_it_has_no_derivative(path, variant, which):
             with pytest.raises(NotImplementedError, match="jvp"):
                 step(state, *token)
             assert not state.window.any()  # refused before anything has happened
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", [contextlib.nullcontext, python_path])
+def test_block_norm_of_overlapping_rows(path):
+    """A sliding window over one line of values: rows closer together than they are long."""
+    D = 40
+    line = torch.randn(200, device="cuda")
+    x, y, gate = line.unfold(0, D, 1)[:50], line.unfold(0, D, 3)[:50], line[100:].unfold(0, D, 1)[:50]
+    w = torch.rand(D, device="cuda")
+    want = block_norm(x.contiguous(), y.contiguous(), w, gate=gate.contiguous())
+    with path():
+        equal(block_norm(x, y, w, gate=gate), want)
+        h = block_norm(x, None, w)[1]
+        assert torch.equal(h, block_norm(x.contiguous(), None, w)[1])
+        leaf = line.clone().requires_grad_(True)
+        z, _ = block_norm(leaf.unfold(0, D, 1)[:50], y, w)
+        (g,) = torch.autograd.grad(z.sum(), leaf)
+    hits = torch.zeros(200, device="cuda").index_add_(0, torch.arange(200, device="cuda").unfold(0, D, 1)[:50].flatten(),
+                                                      torch.ones(50 * D, device="cuda"))
+    assert torch.equal(g, hits)
