@@ -27,7 +27,7 @@ def _option(a, name, value, rows, device, dtypes, cast):
     if not isinstance(value, torch.Tensor):
         try:
             setattr(a, name + "_all", cast(value))
-        except (TypeError, ValueError):
+        except (TypeError, ValueError, OverflowError):
             raise TypeError(f"{name} must be a number, a tensor [{rows}] or None, got {value!r}") from None
         return
     if value.ndim != 1 or value.shape[0] != rows or value.dtype not in dtypes or not value.is_contiguous():
@@ -36,6 +36,11 @@ def _option(a, name, value, rows, device, dtypes, cast):
     if value.device != device:
         raise ValueError("all sampling tensors must share one CUDA device")
     setattr(a, name, value.data_ptr())
+
+
+def _whole(value):
+    """A whole number as 64 bits hold it: what is beyond (a top_k of every token) must not wrap around."""
+    return max(-1, min(int(value), 2**62))
 
 
 def sample(logits, noise, *, temperature=1.0, top_k=None, top_p=None, min_p=None):
@@ -66,7 +71,7 @@ def sample(logits, noise, *, temperature=1.0, top_k=None, top_p=None, min_p=None
     a = N.KdnSampleArgs()
     a.rows, a.V = rows, V
     _option(a, "temperature", temperature, rows, device, (torch.float32,), float)
-    _option(a, "top_k", 0 if top_k is None else top_k, rows, device, (torch.int32, torch.int64), int)
+    _option(a, "top_k", 0 if top_k is None else top_k, rows, device, (torch.int32, torch.int64), _whole)
     _option(a, "top_p", 1.0 if top_p is None else top_p, rows, device, (torch.float32,), float)
     _option(a, "min_p", 0.0 if min_p is None else min_p, rows, device, (torch.float32,), float)
     if not logits.is_cuda:

@@ -328,3 +328,14 @@ def test_hot_rows(T, options):
         assert token[i].item() == at[want], i
         assert abs(prob[i].item() - p) <= 1e-5 * p, i
     assert unclear <= 1
+
+
+@pytest.mark.gpu
+def test_whole_batch_top_k_beyond_64_bits():
+    logits, noise = make(64, 500, seed=30)
+    l, n = logits.cuda(), noise.cuda()
+    want, _ = sample(l, n)
+    for k in (2**31, 2**63, 2**64 + 1, 10**30, -2**64 + 1):
+        assert torch.equal(sample(l, n, top_k=k)[0], want), k
+    with pytest.raises(TypeError, match="top_k must be"):
+        sample(l, n, top_k=math.inf)
