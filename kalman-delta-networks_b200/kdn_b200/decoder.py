@@ -165,7 +165,13 @@ class KDNDecoder(nn.Module):
     def generate(self, prompts, count, *, generator=None, graph=True, **options):
         """``count`` tokens after every row of prompts [B, T]; options as :func:`~kdn_b200.sampling.sample` takes them.
         Returns (tokens [B, count], their probabilities [B, count]); -1 and 0 where a row's logits are all NaN or -inf."""
+        if prompts.ndim != 2 or prompts.shape[1] < 1:
+            raise ValueError(f"prompts must be [B, T] with T >= 1, got {tuple(prompts.shape)}")
+        if count < 0:
+            raise ValueError(f"count must not be negative, got {count}")
         B = prompts.shape[0]
+        if count == 0:
+            return prompts.new_empty((B, 0), dtype=torch.int64), prompts.new_empty((B, 0), dtype=torch.float32)
         pools, steps = self.make_pools(B), [m.make_step() for m in self.mixers]
         slots = torch.arange(B, dtype=torch.int32, device=prompts.device)
         logits = self.start(prompts, pools, slots.long())

@@ -90,3 +90,25 @@ def test_rows_without_a_token_go_on(variant):
     for graph in (True, False):
         tokens, probs = model.generate(prompts, 6, graph=graph, top_k=3)
         assert tokens.shape == (3, 6) and (tokens == -1).all() and (probs == 0).all()
+
+
+def test_no_new_tokens_and_empty_prompts():
+    model = KDNDecoder(16, 128, 1, 1, device="cpu")
+    prompts = torch.zeros(3, 5, dtype=torch.int64)
+    tokens, probs = model.generate(prompts, 0)
+    assert tokens.shape == probs.shape == (3, 0) and tokens.dtype == torch.int64 and probs.dtype == torch.float32
+    with pytest.raises(ValueError, match="count"):
+        model.generate(prompts, -1)
+    with pytest.raises(ValueError, match="prompts must be"):
+        model.generate(prompts[:, :0], 4)
+    with pytest.raises(ValueError, match="prompts must be"):
+        model.generate(prompts[0], 4)
+
+
+@pytest.mark.gpu
+def test_one_new_token():
+    model = make("iso", seed=6)
+    prompts = torch.randint(VOCAB, (2, 1), device="cuda")
+    tokens, probs = model.generate(prompts, 1, temperature=0.0)
+    with torch.no_grad():
+        assert torch.equal(tokens[:, 0], model(prompts)[:, -1].float().argmax(-1)) and (probs == 1).all()
