@@ -7,9 +7,12 @@ missing.  There is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import glob
 import importlib.util
 import os
+import sysconfig
 import threading
+import warnings
 
 import torch
 
@@ -237,25 +240,37 @@ def stream_of(t: torch.Tensor) -> int:
 
 _HOST_ENTRIES = ("kdn_step", "kdn_block_norm_fwd", "kdn_block_norm_bwd", "kdn_block_norm_workspace_bytes", "kdn_sample",
                  "kdn_last_error")
+# Named after the torch and the interpreter it is built against: a library of others is never loaded.
+HOST_LIB = os.path.join(_HERE, "lib", f"_kdn_torch.{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so")
 _host = None
+
+
+def _load_host():
+    if not os.path.exists(HOST_LIB):
+        others = glob.glob(os.path.join(glob.escape(os.path.dirname(HOST_LIB)), "_kdn_torch.*.so"))
+        if others:
+            warnings.warn(f"kdn_b200: the C++ host path is built for another torch or Python ({os.path.basename(others[0])}); "
+                          "taking the Python path until `python -m kdn_b200.build` has run")
+        return None
+    try:
+        spec = importlib.util.spec_from_file_location("_kdn_torch", HOST_LIB)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+    except (ImportError, OSError) as e:
+        warnings.warn(f"kdn_b200: the C++ host path does not load ({e}); taking the Python path")
+        return None
+    lib = load_library()
+    module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _HOST_ENTRIES))
+    return module
 
 
 def host():
     """The C++ host path of the token step, the block norms and the sampling (``csrc/host/kdn_torch.cpp``): their
-    functions answer None for what they leave to the Python path.  None where it is not built, or with
-    ``KDN_B200_HOST=python``; both paths make the same calls into the C library."""
+    functions answer None for what they leave to the Python path.  None where it is not built or does not load (with one
+    warning), or with ``KDN_B200_HOST=python``; both paths make the same calls into the C library."""
     global _host
     if _host is None:
-        path = os.path.join(_HERE, "lib", "_kdn_torch.so")
-        if os.environ.get("KDN_B200_HOST", "") == "python" or not os.path.exists(path):
-            _host = False
-        else:
-            spec = importlib.util.spec_from_file_location("_kdn_torch", path)
-            module = importlib.util.module_from_spec(spec)
-            spec.loader.exec_module(module)
-            lib = load_library()
-            module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _HOST_ENTRIES))
-            _host = module
+        _host = (None if os.environ.get("KDN_B200_HOST", "") == "python" else _load_host()) or False
     return _host or None
 
 

@@ -2,9 +2,9 @@
 
 Each translation unit is compiled in parallel to ``_build/*.o`` and linked
 into one shared library exporting the C ABI declared in ``include/kdn_b200.h``.
-Beside it g++ builds ``lib/_kdn_torch.so`` from ``csrc/host``: the C++ host
-path of the serving operators (``_native.host``).  Rebuilds only when a source
-or header is newer than the libraries.
+Beside it g++ builds ``lib/_kdn_torch.<torch>.<python>.so`` from ``csrc/host``:
+the C++ host path of the serving operators (``_native.host``), one per torch and
+interpreter.  Rebuilds only when a source or header is newer than the libraries.
 
     python -m kdn_b200.build [--force]
 """
@@ -17,12 +17,13 @@ import shutil
 import subprocess
 import sys
 
+from ._native import HOST_LIB
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libkdn_b200.so")
 HOST_SRC = os.path.join(CSRC, "host", "kdn_torch.cpp")
-HOST_LIB = os.path.join(LIB_DIR, "_kdn_torch.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 INCLUDE = os.path.abspath(os.path.join(HERE, "..", "..", "include"))
 

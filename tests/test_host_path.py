@@ -1,6 +1,7 @@
 """The two host paths of the serving operators (``csrc/host/kdn_torch.cpp`` and the Python one behind it) make the
 same C calls: equal outputs, gradients and refusals."""
 import contextlib
+import os
 
 import pytest
 import torch
@@ -235,3 +236,23 @@ def test_block_norm_of_overlapping_rows(path):
     hits = torch.zeros(200, device="cuda").index_add_(0, torch.arange(200, device="cuda").unfold(0, D, 1)[:50].flatten(),
                                                       torch.ones(50 * D, device="cuda"))
     assert torch.equal(g, hits)
+
+
+def test_host_library_of_another_torch_or_broken(tmp_path, monkeypatch):
+    """Never loaded, one warning, and the Python path."""
+    import warnings
+
+    from kdn_b200 import build
+
+    assert torch.__version__ in os.path.basename(build.HOST_LIB)
+    monkeypatch.delenv("KDN_B200_HOST", raising=False)
+    ours = tmp_path / "_kdn_torch.2.0.abi.so"
+    monkeypatch.setattr(N, "HOST_LIB", str(ours))
+    for name, match in (("_kdn_torch.1.9.abi.so", "another torch"), (ours.name, "does not load")):
+        (tmp_path / name).write_bytes(b"not a library")
+        monkeypatch.setattr(N, "_host", None)
+        with pytest.warns(UserWarning, match=match):
+            assert N.host() is None
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            assert N.host() is None
