@@ -256,3 +256,28 @@ def test_host_library_of_another_torch_or_broken(tmp_path, monkeypatch):
         with warnings.catch_warnings():
             warnings.simplefilter("error")
             assert N.host() is None
+
+
+def test_build_without_a_host_compiler(tmp_path, monkeypatch):
+    from kdn_b200 import build
+
+    stale = tmp_path / "_kdn_torch.so"
+    stale.write_bytes(b"of an older source")
+    kernels = []
+    monkeypatch.setattr(build, "HOST_LIB", str(stale))
+    monkeypatch.setattr(build, "up_to_date", lambda: False)
+    monkeypatch.setattr(build, "host_up_to_date", lambda: False)
+    monkeypatch.setattr(build, "_build_kernels", lambda verbose: kernels.append(1))
+    monkeypatch.setattr(build, "_nvcc", lambda: "/usr/local/cuda/bin/nvcc")
+    monkeypatch.setenv("PATH", str(tmp_path))
+    with pytest.warns(UserWarning, match="host path is not built"):
+        assert build.build() == build.LIB
+    assert kernels and not stale.exists()
+    monkeypatch.setattr(build, "host_up_to_date", lambda: True)
+
+    def fails(verbose):
+        raise RuntimeError("nvcc failed")
+
+    monkeypatch.setattr(build, "_build_kernels", fails)
+    with pytest.raises(RuntimeError, match="nvcc failed"):  # the kernels are needed
+        build.build()
