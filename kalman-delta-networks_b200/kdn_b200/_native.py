@@ -15,6 +15,7 @@ import threading
 import warnings
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("KDN_B200_LIB", os.path.join(_HERE, "lib", "libkdn_b200.so"))
@@ -272,6 +273,11 @@ def host():
     if _host is None:
         _host = (None if os.environ.get("KDN_B200_HOST", "") == "python" else _load_host()) or False
     return _host or None
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether a tensor carries a forward-mode derivative (asked tensor by tensor only inside a dual level)."""
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def launch(entry, args, t: torch.Tensor, what: str) -> None:

@@ -17,7 +17,6 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -33,8 +32,8 @@ def _rows(t, D):
     one).  ``empty_like`` of it is contiguous, whatever the rows' stride."""
     if t.ndim != 2:
         t = t.reshape(-1, D)
-    apart = t.shape[0] <= 1 or t.stride(0) >= D or t.stride(0) == 0
-    return t if apart and t.stride(1) == 1 else t.contiguous()
+    apart, inner = t.stride()
+    return t if inner == 1 and (apart >= D or apart == 0 or t.shape[0] <= 1) else t.contiguous()
 
 
 def _args(x, y, gate, weight, post_weight, scale, z, h, rstd, alpha, swish, eps):
@@ -158,8 +157,7 @@ def block_norm(x, y, weight, *, post_weight=None, gate=None, scale=None, alpha=1
     g2 = None if gate is None else _rows(gate, D)
     leaves = [t for t in (x, y, gate, weight, post_weight, scale) if t is not None]
     # forward-mode tangents go to the function too: it refuses them (no jvp) instead of dropping them
-    if (torch.is_grad_enabled() and any([t.requires_grad for t in leaves])) or any(
-            [forward_ad.unpack_dual(t).tangent is not None for t in leaves]):
+    if (torch.is_grad_enabled() and any([t.requires_grad for t in leaves])) or N.has_tangent(*leaves):
         weight, post_weight, scale = [None if w is None else w.contiguous() for w in (weight, post_weight, scale)]
         z, h = _BlockNormFunction.apply(x2, y2, g2, weight, post_weight, scale, alpha, swish, eps)
         if y is None and not x.requires_grad:

@@ -26,7 +26,6 @@ import math
 from numbers import Real
 
 import torch
-from torch.autograd import forward_ad
 
 from . import _native as N
 from .norm_gated import _ACTIVATIONS
@@ -221,7 +220,7 @@ class _Step:
         if not qkv.is_cuda:
             N.require_cuda(qkv)
         inputs = (qkv, *(t for _, t, _ in rows))
-        if any([forward_ad.unpack_dual(t).tangent is not None for t in inputs]):
+        if N.has_tangent(*inputs):
             raise NotImplementedError("kdn_b200 step: the token step has no jvp (forward-mode derivative)")
         if torch.is_grad_enabled() and any([t.requires_grad for t in inputs]):
             return _StepFunction.apply(lambda: self._launch(state, slots, *inputs), *inputs)
