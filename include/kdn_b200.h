@@ -683,7 +683,8 @@ int kdn_block_norm_bwd(const KdnBlockNormArgs* args, kdn_stream_t stream);
  * so that a kept token is drawn with probability e_i / sum of the kept e.
  * T below 1e-37 (0, negative, NaN): the first of the order, prob 1.  NaN
  * logits count as -inf, +inf as the largest fp32 value; a row with nothing
- * above -inf gives token -1, prob 0.  top_k <= 0: no limit.
+ * above -inf gives token -1, prob 0.  top_k <= 0: no limit.  Equal calls give
+ * equal results; the order of the sum Z depends on rows and on alignment.
  * temperature, top_p, min_p: fp32 [rows] or NULL with the value for all rows
  * beside it; top_k: int32 [rows] (int64 if top_k_i64) or NULL likewise.
  * logits: bf16 (logits_bf16) or fp32, noise fp32, with row strides (elements; 0:

@@ -19,12 +19,17 @@
 // Every race lost drops the winner and what is behind it; after kRaces of them
 // (noise that follows the logits) the end of the kept prefix is bisected
 // instead, so that no row takes more than kRaces + 64 turns.  Rows without
-// top-k and top-p race in step 2.  Sums have a fixed order or are integers.
+// top-k and top-p race in step 2.  Sums have a fixed order or are integers, so
+// that equal calls give equal results; the order of Z follows the split into
+// CTAs, which the number of rows decides, and the rows' alignment.
 //
 // One row of 32000 bf16 logits 10.5 us, 61 rows 16.6, 128 rows of 131072 49
 // (unfiltered 35, greedy 22): the latency of the copy, of three cluster-wide
 // reductions and of the random numbers, twice for large rows (two waves), and
 // the passes' instructions; the logits' bytes alone would take 5 us of the 49.
+// Rows of which eight CTAs hold only a part (more than 786432 bf16 or 393216
+// fp32 logits) read the rest again in every pass: 32 rows of 800000 bf16 logits
+// 119 us unfiltered (23 by bytes), 84 top-k 50, 186 top-p 0.9; one row 41.
 #include <cooperative_groups.h>
 
 #include "kdn_launch.cuh"
@@ -461,7 +466,7 @@ __global__ void __launch_bounds__(kSmThreads, 2) sample_kernel(const __grid_cons
 
 template <class T, bool VEC>
 int sample_launch(const KdnSampleArgs& a, cudaStream_t st) {
-  // A CTA per 64 KB (128 rows of 131072 bf16 logits, mixed filters: 56 us, 32 KB 62 us); more while the rows alone
+  // A CTA per 64 KB (128 rows of 131072 bf16 logits, mixed filters: 49 us, 32 KB 62 us); more while the rows alone
   // leave SMs idle and every CTA still has 2048 tokens.
   int64_t ctas = (a.V * (int64_t)sizeof(T) + kSmChunk - 1) / kSmChunk;
   while (2 * ctas <= kSmCluster && 2 * ctas * a.rows <= 296 && a.V / (2 * ctas) >= 2048) ctas *= 2;

@@ -87,7 +87,8 @@ class KDNState:
 
     def reset(self, slots, initial_precision):
         """Start new sequences at ``slots`` (a tensor or list of slot numbers, or a slice): empty memory and past, covariance
-        ``1 / initial_precision`` ([H], the frontend's output)."""
+        ``1 / initial_precision`` ([H], the frontend's output).  Plain indexing, here and in :meth:`store`: slots outside
+        the pool, which mark idle rows of a step, have to be left out."""
         if tuple(initial_precision.shape) != (self.num_heads,):
             raise ValueError(f"initial_precision must be [{self.num_heads}], got {tuple(initial_precision.shape)}")
         prior = 1.0 / initial_precision.float()
@@ -267,7 +268,7 @@ class IsoKDNStep(_Step):
 
     def __call__(self, state, qkv, decay_raw, omega_r_raw, out_gate, slots=None):
         """One token per row: qkv [B, 3*H*D], decay_raw [B, H*D], omega_r_raw [B, 2*H] (omega | r), out_gate [B, H*D],
-        all of one dtype (bf16 or fp32, the window's), rows contiguous (any row stride); slots [B] int32 / int64
+        all of one dtype (bf16 or fp32, the window's), rows contiguous and apart (or one for all); slots [B] int32 / int64
         (None: row b uses slot b; a slot outside the pool marks an idle row, output zero; no slot twice).
         Returns y [B, H*D] and updates the states in place."""
         fast = N.host()

@@ -9,9 +9,11 @@ given random numbers, in one kernel without a sort.
 Every filter looks at the whole distribution (top-p is not renormalised after
 top-k).  ``noise`` holds independent Exp(1) random numbers
 (``torch.empty(rows, V).exponential_()``): the token is then drawn with
-probability e_i / (sum of the kept e), and equal inputs give equal tokens
-whatever the batch around them.  ``prob`` is the token's probability before
-the filters.
+probability e_i / (sum of the kept e).  Equal calls give equal results.  The
+order in which Z is summed follows the number of rows and their alignment, so
+that the same row in another batch may have another last bit of ``prob``, and
+another token where top_p Z lies within that rounding of a sum of e.  ``prob``
+is the token's probability before the filters.  Neither output has a gradient.
 """
 from __future__ import annotations
 
@@ -46,7 +48,7 @@ def _whole(value):
 def sample(logits, noise, *, temperature=1.0, top_k=None, top_p=None, min_p=None):
     """Draw one token per row; returns ``(token int64 [rows], prob fp32 [rows])``.
 
-    logits [rows, V] bf16 or fp32 and noise [rows, V] fp32 (positive), rows contiguous with any row stride.
+    logits [rows, V] bf16 or fp32 and noise [rows, V] fp32 (positive), rows contiguous, any row stride from V up (or 0).
     temperature, top_p, min_p: numbers or fp32 tensors [rows]; top_k: int or int32 / int64 tensor [rows]; None,
     top_k <= 0 or top_p >= 1: no such filter.  temperature below 1e-37 (0, negative): the most likely token, prob 1.
     NaN logits count as -inf and +inf as the largest fp32 value; a row with nothing above -inf gives token -1, prob 0.

@@ -339,3 +339,20 @@ def test_whole_batch_top_k_beyond_64_bits():
         assert torch.equal(sample(l, n, top_k=k)[0], want), k
     with pytest.raises(TypeError, match="top_k must be"):
         sample(l, n, top_k=math.inf)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("options", [{}, {"top_p": 0.9}, {"top_k": 50, "top_p": 0.8}])
+def test_rows_alone_and_in_a_batch(options):
+    """A row is cut into more parts when few rows are in the call: its sum Z then differs by rounding (positive terms,
+    some 100 additions one after another: 100 * 2^-24 = 6e-6), its token only where that decides."""
+    logits, noise = make(64, 32000, seed=3)
+    token, prob = check(logits, noise, **options)
+    differ = 0
+    for i in range(64):
+        t, p = check(logits[i:i + 1], noise[i:i + 1], **options)
+        if t[0] == token[i]:
+            assert abs(p[0] - prob[i]) <= 6e-6 * prob[i]
+        else:
+            differ += 1
+    assert differ <= 1
